@@ -267,6 +267,46 @@ void malus_adamw_multi(const int64_t* params, const int64_t* grads, const int64_
                        const int64_t* vs, size_t n, float lr, float beta1, float beta2,
                        float eps, float wd, int64_t step, float grad_scale);
 
+/* ---- A language model's last part.  f32 values, i32 or i64 ids.  Out
+ * parameters receive new handles (refcount 1); a null one is a result that is
+ * not wanted and not computed. ---- */
+/* Affine layer norm over the last axis: y = (x - mean) / sqrt(var + eps) *
+ * weight + bias, var the biased one.  weight and bias are [D] or 0 (none).
+ * stats, when wanted, is [rows, 2] = (mean, 1 / sqrt(var + eps)) for the
+ * backward pass; a single token's call passes NULL. */
+int64_t malus_layernorm_affine_fwd(int64_t x, int64_t weight, int64_t bias, float eps, int64_t* stats);
+/* Its VJP: dx, and the sums over all rows dweight = sum dout * xhat and
+ * dbias = sum dout (the same bits every run). */
+void malus_layernorm_affine_bwd(int64_t x, int64_t weight, int64_t stats, int64_t dout, int64_t* dx,
+                                int64_t* dweight, int64_t* dbias);
+/* LM head and softmax cross entropy without the [N, V] logits: x [.., D] with
+ * N rows, weight [V, D] (tied != 0: the embedding) or [D, V] (tied == 0, as
+ * tensor_matmul takes it), N targets.  Returns the loss [1], the mean over the
+ * counted rows of nll = logsumexp(logits) - logits[target]; nll is [N].  A row
+ * whose target is negative is not counted: its nll is 0 and it adds to no
+ * gradient (a target at or past V is treated so too, and reported through
+ * malus_device_error as 4).  Without counted rows the loss is 0.  dx and
+ * dweight are the gradients of the loss (for dout = 1; see tape_record_loss).
+ * V is limited to 262144. */
+int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
+                          int64_t* dweight);
+/* Distillation from a teacher's top logits: logits [N, V], and per row K <= 1024
+ * entries ids [N, K] with teacher logits [N, K].  p = softmax over the row's
+ * entries of teacher / temperature, q = softmax(logits / temperature); kl [N]
+ * is temperature^2 * sum p (log p - log q) and the loss [1] its mean over the
+ * counted rows, those with an entry.  A negative id, or a teacher logit of
+ * -inf, is no entry (an id at or past V is treated so too, and reported
+ * through malus_device_error as 4); an id listed twice counts as both entries.
+ * dlogits is the gradient of the loss (for dout = 1).  V is limited to 262140. */
+int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temperature, int64_t* kl,
+                      int64_t* dlogits);
+/* Tape records of the above.  stats, and the n gradients of a loss with respect
+ * to the n inputs, pass to the tape (released at once while it is paused).
+ * backward() multiplies a loss's gradients by the gradient that reaches the
+ * loss (its seed of 1 needs no multiply). */
+void tape_record_layernorm_affine(int64_t x, int64_t weight, int64_t bias, int64_t out, int64_t stats);
+void tape_record_loss(const int64_t* inputs, const int64_t* grads, size_t n, int64_t out);
+
 /* Data parallelism (one process per GPU, NCCL over NVLink).  nccl_id is the
  * 128-byte ncclUniqueId produced by malus_dp_unique_id on rank 0 and shared
  * out of band.  Returns 0 on success, a negative error otherwise. */

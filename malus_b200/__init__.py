@@ -176,6 +176,12 @@ SIGNATURES: dict[str, tuple] = {
     "__matmul_bwd_b": (i64, [i64, i64, i64]),
     # 4. new in this build
     "malus_adamw_multi": (None, [P_i64, P_i64, P_i64, P_i64, sz, f32, f32, f32, f32, f32, i64, f32]),
+    "malus_layernorm_affine_fwd": (i64, [i64, i64, i64, f32, P_i64]),
+    "malus_layernorm_affine_bwd": (None, [i64, i64, i64, i64, P_i64, P_i64, P_i64]),
+    "malus_linear_xent": (i64, [i64, i64, i64, i32, P_i64, P_i64, P_i64]),
+    "malus_distill": (i64, [i64, i64, i64, f32, P_i64, P_i64]),
+    "tape_record_layernorm_affine": (None, [i64, i64, i64, i64, i64]),
+    "tape_record_loss": (None, [P_i64, P_i64, sz, i64]),
     "malus_dp_unique_id": (i32, [P_u8]),
     "malus_dp_init": (i32, [i32, i32, P_u8, i32]),
     "malus_dp_allreduce_f32": (i32, [vp, sz]),
@@ -274,6 +280,25 @@ class Tensor:
         h = lib.tensor_alloc_gpu(DTYPES[a.dtype], s, n, a.ctypes.data_as(C.c_void_p))
         return Tensor(h)
 
+    @staticmethod
+    def wrap(ptr: int, shape, dtype=np.float32) -> "Tensor":
+        """A handle for caller-owned device memory: contiguous row-major data
+        of `shape` at the device address `ptr`, which must stay alive as long as
+        the handle and, since all work runs on the runtime's own stream
+        (malus_stream), until the work queued on it is done.  Work that another
+        stream still has to do on the memory is the caller's to wait for."""
+        s, n = _shape_arr(shape)
+        return Tensor(load().malus_tensor_wrap(DTYPES[np.dtype(dtype)], ptr, s, n))
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        """The data for another library on the same GPU, without a copy.  It is
+        written on the runtime's stream: wait for that (gpu_barrier) before
+        reading it on another, and keep this object alive meanwhile."""
+        lib = load()
+        return {"shape": self.shape, "typestr": np.dtype(self.dtype).str, "strides": None, "version": 2,
+                "data": (lib.malus_tensor_data(self.h) if 0 not in self.shape else 0, False)}
+
     @property
     def shape(self) -> tuple:
         lib = load()
@@ -343,6 +368,51 @@ def tuple_fields(box: int) -> tuple[int, int]:
     a, b = int(arr[1]), int(arr[2])
     C.CDLL(None).free(C.c_void_p(box))
     return a, b
+
+
+def _out() -> "C.Array":
+    return (C.c_int64 * 1)()
+
+
+def _h(t: "Tensor | None") -> int:
+    return t.h if t is not None else 0
+
+
+def layernorm_affine(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,
+                     stats: bool = True) -> tuple[Tensor, Tensor | None]:
+    """Layer norm over the last axis with weight and bias [D]; returns (y,
+    stats), stats [rows, 2] for layernorm_affine_bwd (None with stats=False)."""
+    st = _out() if stats else None
+    y = load().malus_layernorm_affine_fwd(x.h, _h(weight), _h(bias), eps, st)
+    return Tensor(y), Tensor(st[0]) if stats else None
+
+
+def layernorm_affine_bwd(x: Tensor, weight: Tensor | None, stats: Tensor, dout: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias) of layernorm_affine for the incoming gradient."""
+    dx, dw, db = _out(), _out(), _out()
+    load().malus_layernorm_affine_bwd(x.h, _h(weight), stats.h, dout.h, dx, dw, db)
+    return Tensor(dx[0]), Tensor(dw[0]), Tensor(db[0])
+
+
+def linear_xent(x: Tensor, weight: Tensor, targets: Tensor, tied: bool = True,
+                grad: bool = True) -> tuple[Tensor, Tensor, Tensor | None, Tensor | None]:
+    """Mean softmax cross entropy of the head's logits, which are never kept
+    whole: x [.., D], weight [V, D] (tied) or [D, V], one target per row of x
+    (negative: row left out).  Returns (loss [1], nll [N], dx, dweight), the
+    gradients None with grad=False."""
+    nll, dx, dw = _out(), _out() if grad else None, _out() if grad else None
+    loss = load().malus_linear_xent(x.h, weight.h, targets.h, int(tied), nll, dx, dw)
+    return Tensor(loss), Tensor(nll[0]), Tensor(dx[0]) if grad else None, Tensor(dw[0]) if grad else None
+
+
+def distill(logits: Tensor, ids: Tensor, teacher: Tensor, temperature: float = 1.0,
+            grad: bool = True) -> tuple[Tensor, Tensor, Tensor | None]:
+    """Mean temperature^2 * KL of the teacher's top logits (ids, teacher: [N, K],
+    an id below 0 is no entry) against softmax(logits / temperature).  Returns
+    (loss [1], kl [N], dlogits), dlogits None with grad=False."""
+    kl, dl = _out(), _out() if grad else None
+    loss = load().malus_distill(logits.h, ids.h, teacher.h, temperature, kl, dl)
+    return Tensor(loss), Tensor(kl[0]), Tensor(dl[0]) if grad else None
 
 
 class GPT:

@@ -26,6 +26,8 @@ enum OpTag : int32_t {
   kTExp = 8, kTLog = 9, kTSqrt = 10, kTAbs = 11, kTSum = 12, kTranspose = 13, kTNeg = 14,
   kRedSum = 15, kRedMean = 16, kRedMax = 17, kRedVar = 18, kReshape = 19, kSoftmax = 20,
   kLayernorm = 21, kGeluTag = 22, kCrossEntropy = 23, kEmbedding = 24,
+  // this build's own (not valid as the op_tag of the tape_record_* calls above)
+  kLayernormAffine = 25, kFusedLoss = 26,
 };
 
 enum BwdSlot : int32_t {
@@ -42,6 +44,19 @@ struct Node {
   int64_t output;
   std::vector<int64_t> meta;
 };
+
+// How many of a node's saved handles (the first ones) are differentiable inputs.
+size_t inputs_of(const Node& n) {
+  switch (n.op) {
+    case kLayernorm:       // var_h is not one
+    case kCrossEntropy:    // probs, targets are not
+    case kEmbedding:       // indices are not
+      return 1;
+    case kLayernormAffine: return 3;                   // x, weight, bias (0: none); then stats
+    case kFusedLoss: return n.saved.size() / 2;        // inputs, then their gradients
+    default: return n.saved.size();
+  }
+}
 
 // A leaf gradient not yet evaluated: VJP slot `slot` applied to (dout, a, b),
 // all three retained.
@@ -235,6 +250,30 @@ void tape_record_embedding(int32_t op, int64_t w, int64_t idx, int64_t out) {
   t_tape.nodes.push_back(Node{op, {w, idx}, out, {}});
 }
 
+void tape_record_layernorm_affine(int64_t x, int64_t weight, int64_t bias, int64_t out, int64_t stats) {
+  if (!t_tape.recording) {
+    tensor_release(stats);
+    return;
+  }
+  for (int64_t h : {x, weight, bias, out}) tensor_retain(h);
+  t_tape.nodes.push_back(Node{kLayernormAffine, {x, weight, bias, stats}, out, {}});
+}
+
+void tape_record_loss(const int64_t* inputs, const int64_t* grads, size_t n, int64_t out) {
+  for (size_t i = 0; i < n; ++i)
+    if (!same_shape(inputs[i], grads[i])) panic("tape_record_loss: gradient %zu has not its input's shape", i);
+  if (tb(out)->len != 1) panic("tape_record_loss: the loss has %zu elements, not 1", tb(out)->len);
+  if (!t_tape.recording) {
+    for (size_t i = 0; i < n; ++i) tensor_release(grads[i]);
+    return;
+  }
+  std::vector<int64_t> saved(inputs, inputs + n);
+  saved.insert(saved.end(), grads, grads + n);
+  for (size_t i = 0; i < n; ++i) tensor_retain(inputs[i]);
+  tensor_retain(out);
+  t_tape.nodes.push_back(Node{kFusedLoss, std::move(saved), out, {}});
+}
+
 void tape_register_leaf(int64_t h) { t_tape.leaves.insert(h); }
 void tape_pause(void) { t_tape.recording = false; }
 void tape_resume(void) { t_tape.recording = true; }
@@ -266,10 +305,7 @@ void backward(int64_t loss) {
   std::unordered_set<int64_t> live(T.leaves.begin(), T.leaves.end());
   for (auto& n : nodes) {
     bool any = false;
-    size_t nin = n.saved.size();
-    if (n.op == kLayernorm) nin = 1;        // var_h is not a differentiable input
-    if (n.op == kCrossEntropy) nin = 1;     // probs, targets are not
-    if (n.op == kEmbedding) nin = 1;        // indices are not
+    const size_t nin = inputs_of(n);
     for (size_t i = 0; i < nin; ++i) any |= live.count(n.saved[i]) > 0;
     if (any) live.insert(n.output);
   }
@@ -285,17 +321,18 @@ void backward(int64_t loss) {
     std::unordered_set<int64_t> seen;
     for (size_t i = 0; i < nodes.size(); ++i) {
       const Node& n = nodes[i];
-      size_t nin = n.saved.size();
-      if (n.op == kLayernorm || n.op == kCrossEntropy || n.op == kEmbedding) nin = 1;
+      const size_t nin = inputs_of(n);
       for (size_t k = 0; k < nin; ++k)
         if (dp_is_leaf(n.saved[k]) && seen.insert(n.saved[k]).second) final_after[i].push_back(n.saved[k]);
     }
   }
 
   std::unordered_map<int64_t, int64_t> grads;
+  int64_t seed = 0;
   {
     auto* t = tb(loss);
-    grads.emplace(loss, tensor_alloc_ones_gpu(t->shape, t->ndim));
+    seed = tensor_alloc_ones_gpu(t->shape, t->ndim);
+    grads.emplace(loss, seed);
   }
 
   // A leaf read by exactly one node (and in no data-parallel bucket) gets its
@@ -303,8 +340,7 @@ void backward(int64_t loss) {
   // thunk is evaluated only if something besides it still holds the leaf.
   std::unordered_map<int64_t, int> reads;
   for (auto& n : nodes) {
-    size_t nin = n.saved.size();
-    if (n.op == kLayernorm || n.op == kCrossEntropy || n.op == kEmbedding) nin = 1;
+    const size_t nin = inputs_of(n);
     for (size_t i = 0; i < nin; ++i)
       if (T.leaves.count(n.saved[i])) reads[n.saved[i]]++;
   }
@@ -427,6 +463,26 @@ void backward(int64_t loss) {
         int64_t w = n.saved[0];
         if (!need(w)) break;
         accumulate(grads, w, ((F3)slot(sEmbedding))(w, n.saved[1], dout));
+        break;
+      }
+      case kLayernormAffine: {
+        int64_t x = n.saved[0], w = n.saved[1], b = n.saved[2];
+        int64_t dx = 0, dw = 0, db = 0;
+        malus_layernorm_affine_bwd(x, w, n.saved[3], dout, need(x) ? &dx : nullptr, w && need(w) ? &dw : nullptr,
+                                   b && need(b) ? &db : nullptr);
+        if (dx) accumulate(grads, x, dx);
+        if (dw) accumulate(grads, w, dw);
+        if (db) accumulate(grads, b, db);
+        break;
+      }
+      case kFusedLoss: {
+        const size_t k = n.saved.size() / 2;
+        for (size_t i = 0; i < k; ++i) {
+          int64_t in = n.saved[i], g = n.saved[k + i];
+          if (!need(in)) continue;
+          // against the seed of ones the saved gradient is the result
+          accumulate(grads, in, dout == seed ? alias_of(g) : __broadcast_mul_fwd(g, dout));
+        }
         break;
       }
       default: panic("backward: unhandled op tag %d", n.op);
