@@ -1004,6 +1004,21 @@ CUtensorMap encode_f32_map(int rank, const void* base, const uint64_t* dims, con
   return m;
 }
 
+CUtensorMap encode_f16_map(int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                           const uint32_t* box) {
+  load_encoder();
+  CUtensorMap m;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], es[5];
+  for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; es[i] = 1; }
+  for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
+  CUresult r = g_encode(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, (void*)base, d, st, b, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) panic("cuTensorMapEncodeTiled (half, rank %d) failed (%d)", rank, (int)r);
+  return m;
+}
+
 namespace {
 
 // 3-D f32 map {d0 (contiguous), d1, d2}, box {b0, b1, 1}: K-major tiles use the

@@ -1,0 +1,665 @@
+// f32 GEMM on the half-precision tensor pipe.
+//
+// Each operand row is scaled by a power of two and split into two halves, hi =
+// half_rn(x), lo = half_rn(x - hi): 22 bits of every element within 2^-18 of its
+// row's largest, and an error of at most 2^-40 of that largest for smaller
+// ones.  The product keeps hi*lo + lo*hi + hi*hi (the dropped lo*lo is below
+// 2^-22 of a term).  Against three tf32 products of the same 22 bits this takes
+// half the tensor time and half the operand bytes.
+//
+// The tensor core truncates when it adds into its f32 accumulator (measured
+// with products of known sums: a chain of n additions loses about n * 2e-8 of
+// the magnitude, all in one direction; K = 50304 as one chain is off by 8e-5).
+// So a chain is kept short: within a 64-deep stage the small cross products come
+// first, then the four hi*hi additions, and after every second stage (K = 128)
+// the epilogue warps take the accumulator out of tensor memory and add it,
+// rounding to nearest, to sums in their registers, while the tensor core fills
+// the other accumulator.  That costs no tensor time: 128 rows x 256 columns
+// are read in well under the 3072 cycles the next 128 of K take.
+//
+// Work: 2-CTA clusters, each unit a 256 x 256 tile (one tcgen05.mma of M = 256
+// per k-step, cta_group::2) over all of K or a slice of it.  Each CTA loads its
+// 128 rows of A and 128 of B, both planes, 64 deep: 64 KB a stage, three stages,
+// so an SM takes in 64 KB per 1536 cycles of tensor time.  A single CTA's 128 x
+// 256 tile would take 96 KB per the same time, more than L2 delivers.
+// Warp 0 issues the TMA loads, warp 1 (of rank 0) the MMAs, warps 2-9 hold the
+// sums (a row of 128 columns per thread) and store.
+#include "gemm_f16.cuh"
+#include "tc_common.cuh"
+
+#include <vector>
+
+namespace malus {
+namespace {
+using namespace malus::tc;
+
+constexpr int BM = 128, BN = 256, BK = 64, STAGES = 3;
+constexpr int kTile = 128 * BK * 2;                 // one plane's 128 rows, 64 deep
+constexpr int kStageBytes = 4 * kTile;              // A hi, A lo, B hi, B lo
+constexpr int kChunk = 2;                           // stages per accumulator
+constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int kSmem = STAGES * kStageBytes + 1024 + 256;
+static_assert(kSmem <= 232448, "shared memory");
+
+struct Params {
+  int M, N, K, tiles_m, tiles_n, nst, splits;
+  int a_mn, b_mn;
+  int64_t a_k0, b_k0;
+  const float *a_inv, *b_inv;
+  float inv_all;
+  float* out;          // (split, m, n) at split * sstride + m * ldo + n (trans: + n * ldo + m)
+  int64_t ldo, sstride;
+  int trans, accumulate;
+  const int* count;
+  int inner_m;         // consecutive units walk M (else N)
+  float2* part;
+  float* at;
+  const void* target;
+  int tdt;
+  int32_t* err;
+};
+
+struct Unit { int m0, n0, st_lo, st_hi, split; };
+__device__ __forceinline__ Unit unit_at(const Params& p, int u) {
+  Unit r;
+  const int tile = u / p.splits;
+  r.split = u % p.splits;
+  const int i = p.inner_m ? tile % p.tiles_m : tile / p.tiles_n;
+  const int j = p.inner_m ? tile / p.tiles_m : tile % p.tiles_n;
+  r.m0 = i * 2 * BM;
+  r.n0 = j * BN;
+  r.st_lo = (int)((int64_t)r.split * p.nst / p.splits);
+  r.st_hi = (int)((int64_t)(r.split + 1) * p.nst / p.splits);
+  return r;
+}
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc));
+}
+// half x half -> f32, M = 256 over the pair, N = 256
+__device__ __forceinline__ uint32_t idesc_f16(bool a_mn, bool b_mn) {
+  return (1u << 4) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+         ((uint32_t)((2 * BM) >> 4) << 24);
+}
+// 128-byte swizzle.  K-major: rows of 64 halves, 8-row groups 1 KB apart; a step
+// of 16 in K is 32 bytes.  MN-major: columns in chunks of 64 (8 KB each: 64 rows
+// of K), groups of 8 K rows 1 KB apart; a step of 16 in K is 2 KB.
+__device__ __forceinline__ uint64_t desc_of(uint32_t tile, bool mn) {
+  return mn ? umma_desc(tile, BK * 128, 1024, 2) : umma_desc(tile, 16, 1024, 2);
+}
+
+enum Mode : int { kStore = 0, kLse = 1 };
+
+// The 128 sums acc of row m, columns n0 .. n0 + 127, into the output or the row's statistics.
+template <int MODE>
+__device__ __forceinline__ void finish_row(const Params& p, const Unit& un, float (&acc)[128], int m, int n0,
+                                           float alpha) {
+  if (m >= p.M) return;
+  const float sa = alpha * (p.a_inv ? p.a_inv[m] : 1.0f);
+  if (MODE == kLse) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+      acc[j] = n0 + j < p.N ? acc[j] * sa * p.b_inv[n0 + j] : -INFINITY;
+      mx = fmaxf(mx, acc[j]);
+    }
+    float s = 0.0f;
+    const float mm = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) s += exp2f((acc[j] - mm) * kLog2e);
+    p.part[(int64_t)m * (2 * p.tiles_n) + (n0 >> 7)] = make_float2(mx, s);
+    const int64_t t = p.tdt == MALUS_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
+    if (t >= n0 && t < n0 + 128 && t < p.N) {
+      const int o = (int)(t - n0);
+      float zt = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j == o) zt = acc[j];
+      p.at[m] = zt;
+    }
+    return;
+  }
+  if (p.trans) {   // lanes are neighbours in m: whole 128-byte lines
+    float* o = p.out + (int64_t)un.split * p.sstride + m;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+      const int n = n0 + j;
+      if (n < p.N) {
+        const float v = acc[j] * sa * (p.b_inv ? p.b_inv[n] : 1.0f);
+        float* q = o + (int64_t)n * p.ldo;
+        *q = p.accumulate ? *q + v : v;
+      }
+    }
+    return;
+  }
+  float* o = p.out + (int64_t)un.split * p.sstride + (int64_t)m * p.ldo + n0;
+  const bool vec = ((uintptr_t)o & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < 128; j += 4) {
+    const int n = n0 + j;
+    if (vec && n + 4 <= p.N) {
+      float4 v = make_float4(acc[j] * sa, acc[j + 1] * sa, acc[j + 2] * sa, acc[j + 3] * sa);
+      if (p.b_inv) {
+        v.x *= p.b_inv[n]; v.y *= p.b_inv[n + 1]; v.z *= p.b_inv[n + 2]; v.w *= p.b_inv[n + 3];
+      }
+      float4* q = reinterpret_cast<float4*>(o + j);
+      if (p.accumulate) {
+        const float4 c = *q;
+        v.x += c.x; v.y += c.y; v.z += c.z; v.w += c.w;
+      }
+      *q = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) {
+          const float v = acc[j + i] * sa * (p.b_inv ? p.b_inv[n + i] : 1.0f);
+          o[j + i] = p.accumulate ? o[j + i] + v : v;
+        }
+    }
+  }
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUtensorMap mAl,
+           const __grid_constant__ CUtensorMap mBh, const __grid_constant__ CUtensorMap mBl, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + STAGES * kStageBytes);
+  uint64_t* empty = full + STAGES;
+  uint64_t* accf = empty + STAGES;
+  uint64_t* acce = accf + 2;
+  uint64_t* drain = acce + 2;
+  uint64_t* done = drain + 1;   // every epilogue warp finished reading tensor memory
+  uint32_t* tmem_slot = (uint32_t*)(done + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int grp = (int)(blockIdx.x >> 1), ngrp = (int)(gridDim.x >> 1);
+  const int total = p.tiles_m * p.tiles_n * p.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&accf[b]), 1);
+      mbar_init(smem_u32(&acce[b]), 2 * kEpiWarps);   // both CTAs' epilogues
+    }
+    mbar_init(smem_u32(drain), 1);
+    mbar_init(smem_u32(done), kEpiWarps);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  __syncthreads();
+  cluster_sync_all();   // both CTAs' barriers exist before either signals the other
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int u = grp; u < total && ok; u += ngrp) {
+        const Unit un = unit_at(p, u);
+        const int m0 = un.m0 + (int)rank * BM, n0 = un.n0 + (int)rank * 128;   // this CTA's rows of A and of B
+        for (int st = un.st_lo; st < un.st_hi; ++st, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !mbar_wait(smem_u32(&empty[s]), ((it / STAGES) & 1) ^ 1, abort_flag, p.err, 41)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sp = smem + s * kStageBytes;
+          uint32_t fb = smem_u32(&full[s]);
+          if (rank == 0) mbar_expect_tx(fb, 2 * kStageBytes);   // this CTA's and rank 1's copies
+          fb = cluster_addr(fb, 0);
+          const int ka = (int)p.a_k0 + st * BK, kb = (int)p.b_k0 + st * BK;
+          // K-major boxes are 64 (K) x 128 rows; MN-major boxes 64 columns x 64 (K) x 2 column chunks
+          const int a0 = p.a_mn ? 0 : ka, a1 = p.a_mn ? ka : m0, a2 = p.a_mn ? m0 >> 6 : 0;
+          const int b0 = p.b_mn ? 0 : kb, b1 = p.b_mn ? kb : n0, b2 = p.b_mn ? n0 >> 6 : 0;
+          tma_load_3d_pair(smem_u32(sp), &mAh, fb, a0, a1, a2);
+          tma_load_3d_pair(smem_u32(sp + kTile), &mAl, fb, a0, a1, a2);
+          tma_load_3d_pair(smem_u32(sp + 2 * kTile), &mBh, fb, b0, b1, b2);
+          tma_load_3d_pair(smem_u32(sp + 3 * kTile), &mBl, fb, b0, b1, b2);
+        }
+      }
+      if (*abort_flag) {
+        // Every issued copy must land before the CTA exits.  The pair's copies
+        // count on rank 0's barriers: rank 0 waits for its stages (bounded),
+        // rank 1, which cannot observe its own, waits a fixed 200 us.
+        const uint64_t t0 = gtimer();
+        if (rank != 0) {
+          while (gtimer() - t0 < 200000ull) {}
+        } else {
+          for (uint32_t q = it > (uint32_t)STAGES ? it - STAGES : 0; q < it; ++q)
+            while (!mbar_try(smem_u32(&full[q % STAGES]), (q / STAGES) & 1) && gtimer() - t0 < kWaitNs) {}
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (rank 0) ----------------
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_f16(p.a_mn, p.b_mn);
+      const uint32_t s0 = smem_u32(smem);
+      // descriptors of stage 0; a stage or k-step adds (bytes / 16) to the address field
+      const uint64_t da0 = desc_of(s0, p.a_mn), db0 = desc_of(s0 + 2 * kTile, p.b_mn);
+      const uint32_t ka = p.a_mn ? 2048 / 16 : 32 / 16, kb = p.b_mn ? 2048 / 16 : 32 / 16;
+      constexpr uint32_t kLo = kTile / 16, kStage16 = kStageBytes / 16;
+      uint32_t it = 0, chunk = 0;
+      bool ok = true, issued = false;
+      for (int u = grp; u < total && ok; u += ngrp) {
+        const Unit un = unit_at(p, u);
+        for (int st = un.st_lo; st < un.st_hi && ok; st += kChunk, ++chunk) {
+          const uint32_t b = chunk & 1, v = chunk >> 1;
+          if (v >= 1 && !mbar_wait_cluster(smem_u32(&acce[b]), (v - 1) & 1, abort_flag, p.err, 44)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t dacc = tmem + b * BN;
+          const int end = min(st + kChunk, un.st_hi);
+          for (int q = st; q < end; ++q, ++it) {
+            const int s = it % STAGES;
+            if (!mbar_wait(smem_u32(&full[s]), (it / STAGES) & 1, abort_flag, p.err, 42)) {
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t ah = da0 + (uint64_t)(s * kStage16), bh = db0 + (uint64_t)(s * kStage16);
+            const uint64_t al = ah + kLo, bl = bh + kLo;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) {
+              mma_f16_pair(dacc, al + k * ka, bh + k * kb, idesc, q > st || k > 0 ? 1u : 0u);
+              mma_f16_pair(dacc, ah + k * ka, bl + k * kb, idesc, 1u);
+            }
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) mma_f16_pair(dacc, ah + k * ka, bh + k * kb, idesc, 1u);
+            issued = true;
+            mma_commit_pair_both(smem_u32(&empty[s]));   // frees the stage in both CTAs
+          }
+          if (ok) mma_commit_pair_both(smem_u32(&accf[b]));
+        }
+      }
+      if (issued) {
+        // no MMA or commit of this pair may be in flight past the closing cluster barrier
+        mma_commit_pair(smem_u32(drain));
+        const uint64_t t0 = gtimer();
+        while (!mbar_try(smem_u32(drain), 0) && gtimer() - t0 < kWaitNs) {}
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    // Warp w owns lane quarter w % 4 (32 rows, one per lane) and 128 of the
+    // tile's columns.
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const float alpha = p.inv_all * (p.count ? 1.0f / (float)max(1, *p.count) : 1.0f);
+    uint32_t chunk = 0;
+    bool ok = true;
+    for (int u = grp; u < total && ok; u += ngrp) {
+      const Unit un = unit_at(p, u);
+      float acc[128];
+      for (int st = un.st_lo; st < un.st_hi; st += kChunk, ++chunk) {
+        const uint32_t b = chunk & 1;
+        if (!mbar_wait(smem_u32(&accf[b]), (chunk >> 1) & 1, abort_flag, p.err, 43)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (st == un.st_lo) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) tmem_ld16(tbase + b * BN + c, reinterpret_cast<uint32_t*>(acc + c));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {   // 16 at a time: the sums leave no registers for more
+            uint32_t r[16];
+            tmem_ld16(tbase + b * BN + c, r);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(r[j]);
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acce[b]), 0));
+      }
+      if (!ok) break;
+      finish_row<MODE>(p, un, acc, un.m0 + (int)rank * BM + quarter * 32 + lane, un.n0 + half * 128, alpha);
+      __syncwarp();   // rows past M return early: the next tensor memory load needs the whole warp
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(done));
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  __syncthreads();
+  // rank 0 has drained its MMAs and both CTAs' epilogues and copies are done
+  // before either frees its tensor memory or exits
+  cluster_sync_all();
+  if (warp == 1) {
+    mbar_wait_bounded(smem_u32(done), 0);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// out = sum over the K slices, in slice order, of ws[s][m][n] (row pitch ldw)
+__global__ void k_f16_join(const float* __restrict__ ws, int splits, int64_t sstride, int M, int N, int64_t ldw,
+                           float* __restrict__ out, int64_t ldo, int trans, int accumulate) {
+  const int64_t total = (int64_t)M * N;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t m = trans ? i % M : i / N, n = trans ? i / M : i % N;
+    float s = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += ws[k * sstride + m * ldw + n];
+    float* o = out + (trans ? n * ldo + m : m * ldo + n);
+    *o = accumulate ? *o + s : s;
+  }
+}
+
+// ------------------------------------------------------------------ planes
+// The power of two that brings `m` (a magnitude, its bits) into [2^13, 2^14), as
+// a scale and its inverse; 1 for zero.  Both stay normal numbers.
+__device__ __forceinline__ void scale_for(uint32_t bits, float* up, float* inv) {
+  int e = (int)(bits >> 23) - 127;              // floor(log2), -127 for subnormals
+  int s = bits ? kF16Exp - e : 0;
+  s = s > 126 ? 126 : s < -113 ? -113 : s;
+  *up = __uint_as_float((uint32_t)(s + 127) << 23);
+  *inv = __uint_as_float((uint32_t)(127 - s) << 23);
+}
+__device__ __forceinline__ uint32_t finite_bits(float x) {   // bits of |x|; 0 for inf and NaN
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b >= 0x7f800000u ? 0u : b;
+}
+__device__ __forceinline__ void split2(float x, __half* h, __half* l) {
+  *h = __float2half_rn(x);
+  *l = __float2half_rn(x - __half2float(*h));
+}
+
+// One row per group of G threads (a warp, or a block of 512).
+template <int G, bool VEC>
+__global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* __restrict__ src, int64_t R, int64_t C,
+                                                                  int64_t Cp, __half* __restrict__ hi,
+                                                                  __half* __restrict__ lo, float* __restrict__ inv) {
+  __shared__ uint32_t sh[G / 32];
+  constexpr int PER = G == 32 ? 8 : 1;
+  const int t = threadIdx.x % G;
+  for (int64_t r = (int64_t)blockIdx.x * PER + threadIdx.x / G; r < R; r += (int64_t)gridDim.x * PER) {
+    const float* s = src + r * C;
+    uint32_t m = 0;
+    if (VEC) {
+      for (int64_t c = 4 * t; c < C; c += 4 * G) {
+        const float4 v = *reinterpret_cast<const float4*>(s + c);
+        m = max(m, max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w))));
+      }
+    } else {
+      for (int64_t c = t; c < C; c += G) m = max(m, finite_bits(s[c]));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (G > 32) {
+      if ((t & 31) == 0) sh[t >> 5] = m;
+      __syncthreads();
+      for (int i = 0; i < G / 32; ++i) m = max(m, sh[i]);
+      __syncthreads();
+    }
+    float up, iv;
+    scale_for(m, &up, &iv);
+    if (t == 0) inv[r] = iv;
+    __half *hr = hi + r * Cp, *lr = lo + r * Cp;
+    for (int64_t c = 4 * t; c < Cp; c += 4 * G) {
+      float v[4];
+      if (VEC && c < C) {
+        const float4 q = *reinterpret_cast<const float4*>(s + c);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c + j < C ? s[c + j] : 0.0f;
+      }
+      __align__(8) __half h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split2(v[j] * up, &h[j], &l[j]);
+      *reinterpret_cast<uint2*>(hr + c) = *reinterpret_cast<uint2*>(h);
+      *reinterpret_cast<uint2*>(lr + c) = *reinterpret_cast<uint2*>(l);
+    }
+  }
+}
+
+__device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, int64_t r) {
+  if (!keep) return true;
+  const int64_t t = dt == MALUS_I64 ? ((const int64_t*)keep)[r] : (int64_t)((const int32_t*)keep)[r];
+  return t >= 0 && t < limit;
+}
+
+// bits[c] = largest finite magnitude of column c (as bits; zeroed before):
+// 32 columns x 8 rows per block, a slice of rows per blockIdx.y
+__global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
+                                                 uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
+  __shared__ uint32_t sh[8][32];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  uint32_t m = 0;
+  if (c < C) {
+#pragma unroll 8
+    for (int64_t r = (int64_t)blockIdx.y * 8 + g; r < R; r += (int64_t)gridDim.y * 8)
+      if (kept(keep, kdt, limit, r)) m = max(m, finite_bits(src[r * C + c]));
+  }
+  sh[g][lane] = m;
+  __syncthreads();
+  if (g == 0 && c < C) {
+    for (int i = 1; i < 8; ++i) m = max(m, sh[i][lane]);
+    atomicMax(bits + c, m);   // a maximum: the order does not matter
+  }
+}
+
+// 64 x 64 tiles through shared memory: rows of the source in, columns out.
+__global__ void __launch_bounds__(256) k_split_cols(const float* __restrict__ src, int64_t R, int64_t C, int64_t Rp,
+                                                    const uint32_t* __restrict__ bits, __half* __restrict__ hi,
+                                                    __half* __restrict__ lo, float* __restrict__ inv, const void* keep,
+                                                    int kdt, int64_t limit) {
+  __shared__ float tile[64][65];
+  const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * 64;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int64_t c = c0 + tx;
+  float up = 1.0f, iv = 1.0f;
+  if (c < C) scale_for(bits[c], &up, &iv);
+#pragma unroll
+  for (int i = ty; i < 64; i += 4) {
+    const int64_t r = r0 + i;
+    tile[i][tx] = r < R && c < C && kept(keep, kdt, limit, r) ? src[r * C + c] * up : 0.0f;
+  }
+  if (blockIdx.y == 0 && ty == 0 && c < C) inv[c] = iv;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = w; i < 64; i += 8) {
+    if (c0 + i >= C) continue;
+    __align__(4) __half h[2], l[2];
+    split2(tile[2 * lane][i], &h[0], &l[0]);
+    split2(tile[2 * lane + 1][i], &h[1], &l[1]);
+    const int64_t o = (c0 + i) * Rp + r0 + 2 * lane;
+    *reinterpret_cast<uint32_t*>(hi + o) = *reinterpret_cast<uint32_t*>(h);
+    *reinterpret_cast<uint32_t*>(lo + o) = *reinterpret_cast<uint32_t*>(l);
+  }
+}
+
+// ------------------------------------------------------------------ launch
+CUtensorMap map_of(const F16Operand& o, const __half* plane) {
+  const uint64_t pb = (uint64_t)o.pitch * 2;
+  if (o.mn_major) {
+    const uint64_t dims[3] = {64, (uint64_t)o.rows, (uint64_t)(o.cols + 63) / 64}, st[2] = {pb, 128};
+    const uint32_t box[3] = {64, BK, 2};
+    return encode_f16_map(3, plane, dims, st, box);
+  }
+  const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, 1}, st[2] = {pb, pb * (uint64_t)o.rows};
+  const uint32_t box[3] = {BK, 128, 1};
+  return encode_f16_map(3, plane, dims, st, box);
+}
+
+template <int MODE>
+cudaLaunchConfig_t config(int grid, cudaLaunchAttribute* at) {
+  static bool attr = false;
+  if (!attr) {
+    MALUS_CUDA(cudaFuncSetAttribute(k_gemm_f16<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    attr = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream();
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Pairs resident at once: one per TPC, fewer where the device places fewer.
+int max_pairs() {
+  static int n = [] {
+    cudaLaunchAttribute at[1];
+    cudaLaunchConfig_t cfg = config<kStore>(kNumSMs, at);
+    int c = 0;
+    MALUS_CUDA(cudaOccupancyMaxActiveClusters(&c, k_gemm_f16<kStore>, &cfg));
+    if (c < 1) panic("gemm_f16: no CTA pair can be resident");
+    return std::min(c, kNumSMs / 2);
+  }();
+  return n;
+}
+
+template <int MODE>
+void launch(const F16Gemm& g, Params& p) {
+  p.M = g.M; p.N = g.N; p.K = g.K;
+  p.tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
+  p.tiles_n = (g.N + BN - 1) / BN;
+  p.inner_m = p.tiles_m <= p.tiles_n;
+  p.a_mn = g.a.mn_major; p.b_mn = g.b.mn_major;
+  p.a_k0 = g.a.k0; p.b_k0 = g.b.k0;
+  p.a_inv = g.a.inv; p.b_inv = g.b.inv;
+  p.inv_all = (g.a.inv ? 1.0f : g.a.inv_all) * (g.b.inv ? 1.0f : g.b.inv_all);
+  p.err = device_error_word();
+  const int units = p.tiles_m * p.tiles_n * p.splits;
+  cudaLaunchAttribute at[1];
+  cudaLaunchConfig_t cfg = config<MODE>(2 * std::min(units, max_pairs()), at);
+  const int pid = prof_begin(0, 2.0 * g.M * (double)g.N * g.K,
+                             4.0 * ((double)g.M * g.K + (double)g.N * g.K) + 4.0 * (double)g.M * g.N);
+  MALUS_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_f16<MODE>, map_of(g.a, g.a.hi), map_of(g.a, g.a.lo), map_of(g.b, g.b.hi),
+                                map_of(g.b, g.b.lo), p));
+  count_launch();
+  after_launch("k_gemm_f16");
+  prof_end(pid);
+}
+
+// K slices: the count with the least time in stages of the longest-working pair
+// (a slice costs about 4 stages of its own: the pipeline's fill, its store and
+// its part of the join).
+int splits_for(int tiles, int nst, int pairs) {
+  int best = 1;
+  double best_t = 1e30;
+  for (int s = 1; s <= 64 && s * 4 <= std::max(4, nst); ++s) {
+    const double waves = (double)(((int64_t)tiles * s + pairs - 1) / pairs);
+    const double t = waves * ((double)((nst + s - 1) / s) + 4.0) + (s > 1 ? 4.0 + 0.25 * s : 0.0);
+    if (t < best_t) { best_t = t; best = s; }
+  }
+  return best;
+}
+
+}  // namespace
+
+void gemm_f16(const F16Gemm& g) {
+  if (g.M <= 0 || g.N <= 0) return;
+  if (g.K <= 0) panic("gemm_f16 with K = %d", g.K);
+  Params p{};
+  p.nst = (g.K + BK - 1) / BK;
+  const int tiles = ((g.M + 2 * BM - 1) / (2 * BM)) * ((g.N + BN - 1) / BN);
+  p.splits = splits_for(tiles, p.nst, max_pairs());
+  p.count = g.count;
+  if (p.splits == 1) {
+    p.out = g.out;
+    p.ldo = g.ldo;
+    p.trans = g.trans;
+    p.accumulate = g.accumulate;
+    launch<kStore>(g, p);
+    return;
+  }
+  p.ldo = (g.N + 3) / 4 * 4;
+  p.sstride = (int64_t)g.M * p.ldo;
+  p.out = static_cast<float*>(scratch_alloc((size_t)p.sstride * p.splits * 4));
+  launch<kStore>(g, p);
+  k_f16_join<<<grid_for((size_t)g.M * g.N, 256), 256, 0, stream()>>>(p.out, p.splits, p.sstride, g.M, g.N, p.ldo, g.out,
+                                                                     g.ldo, g.trans, g.accumulate);
+  count_launch();
+  after_launch("k_f16_join");
+  scratch_free(p.out);
+}
+
+int f16_lse_parts(int N) { return 2 * ((N + BN - 1) / BN); }
+
+void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target, int tgt_dtype) {
+  if (g.M <= 0) return;
+  Params p{};
+  p.nst = (g.K + BK - 1) / BK;
+  p.splits = 1;
+  p.part = part;
+  p.at = at;
+  p.target = target;
+  p.tdt = tgt_dtype;
+  launch<kLse>(g, p);
+}
+
+void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv) {
+  if (R == 0) return;
+  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
+  const int64_t Cp = pad64(C);
+  const int pid = prof_begin(1, 0.0, 8.0 * (double)R * (double)C);
+  // a warp per row up to 4096 columns, which its second pass finds in L1
+  if (C <= 4096) {
+    const unsigned grid = (unsigned)std::min<int64_t>((R + 7) / 8, kNumSMs * 8);
+    if (vec) k_split_rows<32, true><<<grid, 256, 0, stream()>>>(src, R, C, Cp, hi, lo, inv);
+    else k_split_rows<32, false><<<grid, 256, 0, stream()>>>(src, R, C, Cp, hi, lo, inv);
+  } else {
+    const unsigned grid = (unsigned)std::min<int64_t>(R, kNumSMs * 4);
+    if (vec) k_split_rows<512, true><<<grid, 512, 0, stream()>>>(src, R, C, Cp, hi, lo, inv);
+    else k_split_rows<512, false><<<grid, 512, 0, stream()>>>(src, R, C, Cp, hi, lo, inv);
+  }
+  count_launch();
+  after_launch("k_split_rows");
+  prof_end(pid);
+}
+
+void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
+                    int keep_dtype, int64_t limit) {
+  if (C == 0) return;
+  const int64_t Rp = pad64(R);
+  uint32_t* bits = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
+  const int pid = prof_begin(1, 0.0, 8.0 * (double)R * (double)C);
+  MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
+  const int64_t cb = (C + 31) / 32;
+  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 63) / 64, (kNumSMs * 16 + cb - 1) / cb));
+  k_col_max<<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  if (Rp / 64 > 65535) panic("f16_split_cols of %lld rows", (long long)R);
+  k_split_cols<<<dim3((unsigned)((C + 63) / 64), (unsigned)(Rp / 64)), 256, 0, stream()>>>(
+      src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
+  count_launch(2);
+  after_launch("k_split_cols");
+  scratch_free(bits);
+  prof_end(pid);
+}
+
+}  // namespace malus

@@ -1,0 +1,54 @@
+// f32 GEMM through three half-precision products (gemm_f16.cu).
+#pragma once
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace malus {
+
+// A matrix of f32 values held as two half planes: value = (hi + lo) * inv, with
+// inv a power of two per row of the product's M or N (or one for all).  Both
+// planes have `pitch` halves per stored row, a multiple of 64, zero past the
+// matrix.  K-major: stored rows are M (or N), columns K.  MN-major: stored rows
+// are K, columns M (or N).
+struct F16Operand {
+  const __half *hi, *lo;
+  int64_t rows, cols, pitch;
+  bool mn_major;
+  int64_t k0;          // first K column read (K-major only; a multiple of 64)
+  const float* inv;    // per M (or N) index; null: inv_all
+  float inv_all;
+};
+
+// out[m * ldo + n] (or out[n * ldo + m] with trans) = A B^T / max(1, count[0])
+// (count null: as it is), added to what is there with accumulate.
+struct F16Gemm {
+  int M, N, K;
+  F16Operand a, b;
+  float* out;
+  int64_t ldo;
+  bool trans, accumulate;
+  const int* count;
+};
+void gemm_f16(const F16Gemm& g);
+
+// Row statistics of A B^T without storing it: part[m * parts + i] = (maximum,
+// sum of exp(value - maximum)) over the i-th 128 columns, parts =
+// f16_lse_parts(N), and at[m] = the value in column target[m] (rows whose target
+// lies outside [0, N) get none).
+int f16_lse_parts(int N);
+void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target, int tgt_dtype);
+
+// Planes of a row-major R x C matrix: its rows (hi/lo [R][pad64(C)], inv[R]), or
+// its columns (hi/lo [C][pad64(R)], inv[C]).  Each plane row is scaled by the
+// power of two that brings its largest finite magnitude into [2^13, 2^14).
+// keep (columns only, may be null): rows whose keep id lies outside [0, limit)
+// are taken as zeros.
+void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv);
+void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
+                    int keep_dtype, int64_t limit);
+inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+
+constexpr int kF16Exp = 13;   // scaled magnitudes stay below 2^(kF16Exp + 1)
+
+}  // namespace malus

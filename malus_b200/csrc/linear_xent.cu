@@ -4,16 +4,93 @@
 //   logits = x W^T,  nll = logsumexp(logits) - logits[target]
 //   dl = (softmax(logits) - onehot(target)) / rows,  dx = dl W,  dW = dl^T x
 //
-// Tokens are taken in pieces: a piece's logits live in a scratch of at most
-// kPieceBytes, become dl in place, feed both gradient products and make room
-// for the next piece.  Training costs the three products (6 N D V flops) and
-// nothing is computed twice.
+// Training takes the tokens in pieces: a piece's logits live in a scratch of at
+// most kPieceBytes, become the half planes of dl in place (loss_rows.cu), feed
+// both gradient products and make room for the next piece.  That is the three
+// products (6 N D V flops) and nothing computed twice; the scratch costs 4 B
+// written and read per logit, then 4 B written and read by each product.  The
+// loss alone stores no logits: the product's epilogue reduces each row of a tile
+// to its maximum, sum of exponentials and target logit.
+//
+// All products run as three half-precision ones (gemm_f16.cuh).  x and weight
+// are split twice, by rows and by columns, so that every product's operands are
+// scaled along the axis it does not sum over.
+#include "gemm_f16.cuh"
 #include "loss_rows.cuh"
 
 namespace malus {
 namespace {
 
 constexpr size_t kPieceBytes = (size_t)512 << 20;
+// rows per statistics buffer of the loss alone (8 B per 128 logits)
+constexpr size_t kLossRows = (size_t)1 << 18;
+
+// Half planes of an operand, in one scratch block with their scales.
+struct Planes {
+  __half *hi, *lo;
+  float* inv;
+  int64_t rows, pitch;
+  Planes(int64_t r, int64_t cols) : rows(r), pitch(pad64(cols)) {
+    const size_t plane = (size_t)rows * pitch;
+    hi = static_cast<__half*>(scratch_alloc(plane * 4 + (size_t)rows * 4));
+    lo = hi + plane;
+    inv = reinterpret_cast<float*>(lo + plane);
+  }
+  ~Planes() { scratch_free(hi); }
+  Planes(const Planes&) = delete;
+  // rows [r0, r0 + n), read along K from column k0
+  F16Operand kmajor(int64_t r0, int64_t n, int64_t k0 = 0) const {
+    return {hi + r0 * pitch, lo + r0 * pitch, n, pitch, pitch, false, k0, inv + r0, 1.0f};
+  }
+};
+
+void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
+           int64_t ld, const Planes& wv, const Planes& xr, const int* count, float* nll, float* dx, float* dw) {
+  // x by columns, tokens that are not counted as zeros: whatever they hold, dl
+  // is 0 there; weight by columns (tied) or rows: an embedding axis per row
+  Planes xc(dw ? D : 0, n), wd(dx ? D : 0, V);
+  if (dw) f16_split_cols(x, n, D, xc.hi, xc.lo, xc.inv, tgt, tdt, V);
+  if (dx && tied) f16_split_cols(w, V, D, wd.hi, wd.lo, wd.inv, nullptr, 0, 0);
+  if (dx && !tied) f16_split_rows(w, D, V, wd.hi, wd.lo, wd.inv);
+  // pieces of whole 256-row tiles, of even size
+  const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * 4)) / 256 * 256);
+  const int64_t pieces = (n + most - 1) / most;
+  const int64_t piece = ((n + pieces - 1) / pieces + 255) / 256 * 256;
+  float* logits = static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
+  const __half* hi = reinterpret_cast<const __half*>(logits);
+  constexpr float inv = 1.0f / (1 << kF16Exp);
+  for (int64_t r0 = 0; r0 < n; r0 += piece) {
+    const int64_t m = std::min(piece, n - r0);
+    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), logits, ld, false, false, nullptr};
+    gemm_f16(g);
+    xent_rows(logits, ld, m, V, tgt, tdt, r0, nll);
+    if (dx) {
+      const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, false, 0, nullptr, inv};
+      gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, false, count});
+    }
+    if (dw) {
+      const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, true, 0, nullptr, inv};
+      gemm_f16({(int)V, (int)D, (int)m, dl, xc.kmajor(0, D, r0), dw, tied ? D : V, !tied, r0 > 0, count});
+    }
+  }
+  scratch_free(logits);
+}
+
+void loss_only(const void* tgt, int tdt, int64_t n, int64_t D, int64_t V, const Planes& wv, const Planes& xr,
+               float* nll) {
+  const int parts = f16_lse_parts((int)V);
+  const int64_t piece = std::min<int64_t>(n, kLossRows);
+  float2* part = static_cast<float2*>(scratch_alloc((size_t)piece * (parts * 8 + 4)));
+  float* at = reinterpret_cast<float*>(part + piece * parts);
+  for (int64_t r0 = 0; r0 < n; r0 += piece) {
+    const int64_t m = std::min(piece, n - r0);
+    const void* t = static_cast<const char*>(tgt) + r0 * (int64_t)dtype_size(tdt);
+    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), nullptr, 0, false, false, nullptr};
+    gemm_f16_lse(g, part, at, t, tdt);
+    xent_join(part, parts, at, t, tdt, V, m, nll + r0);
+  }
+  scratch_free(part);
+}
 
 }  // namespace
 }  // namespace malus
@@ -45,45 +122,20 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
   const void* tp = vptr(targets);
   const int64_t loss = alloc_f32({1}), hn = alloc_f32({n});
   const int64_t hx = dx ? alloc_shape(sx) : 0, hw = dweight ? alloc_shape(sw) : 0;
-  const bool grad = hx || hw;
   int* count = static_cast<int*>(scratch_alloc(4));
   xent_count(tp, tdt, (int64_t)n, (int64_t)V, count);
-  const size_t piece = std::max<size_t>(64, std::min<size_t>((n + 63) / 64 * 64, kPieceBytes / (ld * 4) / 64 * 64));
-  float* logits = static_cast<float*>(scratch_alloc(piece * ld * 4));
-  for (size_t r0 = 0; r0 < n; r0 += piece) {
-    const int m = (int)std::min(piece, n - r0);
-    const GemmOperand X = plain_operand(xp + r0 * D, 1, m, D, D, 0);
-    const GemmOperand W = plain_operand(wp, 1, sw.d[0], sw.d[1], sw.d[1], 0);
-    const GemmOperand L = plain_operand(logits, 1, m, V, ld, 0);
-    GemmArgs g{};
-    g.M = m; g.N = (int)V; g.K = (int)D; g.batch = 1;
-    g.A = X; g.B = W; g.b_trans = tied != 0;
-    g.C = logits; g.ldc = ld;
-    gemm(g);
-    xent_rows(logits, ld, m, (int64_t)V, tp, tdt, (int64_t)r0, fptr(hn), grad);
-    if (hx) {
-      GemmArgs q{};
-      q.M = m; q.N = (int)D; q.K = (int)V; q.batch = 1;
-      q.A = L; q.B = W; q.b_trans = tied == 0;
-      q.C = fptr(hx) + r0 * D; q.ldc = D;
-      gemm(q);
-    }
-    if (hw) {
-      GemmArgs q{};
-      q.K = m; q.batch = 1;
-      q.a_trans = true;
-      if (tied) { q.M = (int)V; q.N = (int)D; q.A = L; q.B = X; }
-      else { q.M = (int)D; q.N = (int)V; q.A = X; q.B = L; }
-      q.C = fptr(hw); q.ldc = q.N;
-      q.beta = r0 ? 1.0f : 0.0f;
-      gemm(q);
-    }
-  }
-  scratch_free(logits);
-  if (hx && n) scale_by_count(fptr(hx), n * D, count);
-  if (hw) {
-    if (n) scale_by_count(fptr(hw), V * D, count);
-    else MALUS_CUDA(cudaMemsetAsync(fptr(hw), 0, V * D * 4, stream()));
+  if (n == 0) {
+    if (hw) MALUS_CUDA(cudaMemsetAsync(fptr(hw), 0, V * D * 4, stream()));
+  } else {
+    const int64_t N = (int64_t)n;
+    Planes wv(V, D);   // a vocabulary entry per row
+    if (tied) f16_split_rows(wp, V, D, wv.hi, wv.lo, wv.inv);
+    else f16_split_cols(wp, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
+    Planes xr(N, D);   // a token per row
+    f16_split_rows(xp, N, D, xr.hi, xr.lo, xr.inv);
+    if (hx || hw) train(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, ld, wv, xr, count, fptr(hn),
+                        hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
+    else loss_only(tp, tdt, N, (int64_t)D, (int64_t)V, wv, xr, fptr(hn));
   }
   loss_mean(fptr(hn), (int64_t)n, count, fptr(loss));
   scratch_free(count);

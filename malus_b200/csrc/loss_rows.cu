@@ -8,6 +8,7 @@
 // cluster of up to 8 that exchange their maximum and sum through distributed
 // shared memory, so the gradient row is written without reading the logits
 // again (4 B read and 4 B written per logit).
+#include "gemm_f16.cuh"
 #include "loss_rows.cuh"
 
 #include <cooperative_groups.h>
@@ -131,9 +132,26 @@ __device__ __forceinline__ RowStat row_stat(float4 (&v)[kNV], int n, float c, cg
   return {M, S};
 }
 
+// Four elements of the row's gradient, magnitudes at most 1, as the half planes
+// that the head's products read: hi in the first half of the row's memory, lo in
+// the second.
+__device__ __forceinline__ void store_planes(float* row, int64_t ld, int64_t e, float4 q) {
+  constexpr float up = (float)(1 << kF16Exp);
+  const float x[4] = {q.x * up, q.y * up, q.z * up, q.w * up};
+  __align__(8) __half h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = __float2half_rn(x[j]);
+    l[j] = __float2half_rn(x[j] - __half2float(h[j]));
+  }
+  __half* p = reinterpret_cast<__half*>(row);
+  *reinterpret_cast<uint2*>(p + e) = *reinterpret_cast<uint2*>(h);
+  *reinterpret_cast<uint2*>(p + ld + e) = *reinterpret_cast<uint2*>(l);
+}
+
 __global__ void __launch_bounds__(kMaxThreads)
 k_xent_rows(float* __restrict__ logits, int64_t ld, int64_t V, const void* __restrict__ tgt, int tdt, int64_t row0,
-            float* __restrict__ nll, int grad) {
+            float* __restrict__ nll) {
   __shared__ float red[64];
   __shared__ float2 mine;
   cg::cluster_group cl = cg::this_cluster();
@@ -158,7 +176,6 @@ k_xent_rows(float* __restrict__ logits, int64_t ld, int64_t V, const void* __res
     }
     const RowStat st = row_stat(v, n, kLog2e, cl, red, &mine);
     if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
-    if (!grad) return;
     const float inv = 1.0f / st.sum;
 #pragma unroll
     for (int k = 0; k < kNV; ++k)
@@ -171,13 +188,12 @@ k_xent_rows(float* __restrict__ logits, int64_t ld, int64_t V, const void* __res
           if (t == e + 2) q.z -= 1.0f;
           if (t == e + 3) q.w -= 1.0f;
         }
-        *reinterpret_cast<float4*>(row + e) = q;   // columns from V on hold exp(-inf) = 0
+        store_planes(row, ld, e, q);   // columns from V on hold exp(-inf) = 0
       }
   } else {
     if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = 0.0f;
-    if (!grad) return;
     for (int64_t g = sl.g0 + threadIdx.x; g < sl.g1; g += blockDim.x)
-      *reinterpret_cast<float4*>(row + 4 * g) = make_float4(0.f, 0.f, 0.f, 0.f);
+      store_planes(row, ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
   }
 }
 
@@ -219,10 +235,29 @@ __global__ void __launch_bounds__(1024) k_loss_mean(const float* __restrict__ v,
   }
 }
 
-__global__ void k_scale_by_count(float* __restrict__ v, int64_t n, const int* __restrict__ count) {
-  const float f = 1.0f / (float)max(1, count[0]);
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    v[i] *= f;
+// nll of a row from its parts' (maximum, sum of exponentials) and its target's
+// logit; a warp per row
+__global__ void __launch_bounds__(256) k_xent_join(const float2* __restrict__ part, int parts,
+                                                   const float* __restrict__ at, const void* __restrict__ tgt, int tdt,
+                                                   int64_t V, int64_t n, float* __restrict__ nll) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += (int64_t)gridDim.x * 8) {
+    const int64_t t = id_at(tgt, tdt, r);
+    if (t < 0 || t >= V) {
+      if (lane == 0) nll[r] = 0.0f;
+      continue;
+    }
+    float M = -INFINITY;
+    for (int i = lane; i < parts; i += 32) M = fmaxf(M, part[r * parts + i].x);
+    M = wmax(M);
+    float s = 0.0f;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 o = part[r * parts + i];
+      s += o.y * (o.x == -INFINITY ? 1.0f : exp2f((o.x - M) * kLog2e));   // -inf only: the sum is 0 or NaN
+    }
+    s = wsum(s);
+    if (lane == 0) nll[r] = logf(s) - (at[r] - M);
+  }
 }
 
 // ---- distillation ----
@@ -408,21 +443,23 @@ void xent_count(const void* targets, int tgt_dtype, int64_t n, int64_t V, int* c
 }
 
 void xent_rows(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, int64_t row0,
-               float* nll, bool grad) {
+               float* nll) {
   if (n == 0) return;
   int cs, threads;
   if (!row_launch(ld / 4, &cs, &threads)) panic("xent_rows: rows of %lld logits", (long long)V);
-  const int pid = prof_begin_named("k_xent_rows", (grad ? 8.0 : 4.0) * (double)n * (double)ld);
-  launch_rows(k_xent_rows, n, cs, threads, 0, logits, ld, V, targets, tgt_dtype, row0, nll, grad ? 1 : 0);
+  const int pid = prof_begin_named("k_xent_rows", 8.0 * (double)n * (double)ld);
+  launch_rows(k_xent_rows, n, cs, threads, 0, logits, ld, V, targets, tgt_dtype, row0, nll);
   count_launch();
   after_launch("k_xent_rows");
   prof_end(pid);
 }
 
-void scale_by_count(float* v, int64_t n, const int* count) {
-  k_scale_by_count<<<grid_for((size_t)n, 256), 256, 0, stream()>>>(v, n, count);
+void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,
+               float* nll) {
+  if (n == 0) return;
+  k_xent_join<<<grid_for((size_t)n * 32, 256), 256, 0, stream()>>>(part, parts, at, targets, tgt_dtype, V, n, nll);
   count_launch();
-  after_launch("k_scale_by_count");
+  after_launch("k_xent_join");
 }
 
 void loss_mean(const float* v, int64_t n, const int* count, float* loss) {

@@ -10,15 +10,17 @@ namespace malus {
 // in the runtime's error word (and its row left out, as a negative one's).
 void xent_count(const void* targets, int tgt_dtype, int64_t n, int64_t V, int* count);
 
-// Rows [0, n) of f32 logits (row pitch ld >= V, a multiple of 4) against targets[row0 ..]:
-//   nll[row0 + r] = logsumexp - logits[target]   (0 for rows left out)
-// and, with grad, the row in place becomes (softmax - onehot) (0 for rows left
-// out and for the columns from V to ld).
+// Rows [0, n) of f32 logits (row pitch ld >= V, a multiple of 64) against
+// targets[row0 ..]: nll[row0 + r] = logsumexp - logits[target] (0 for rows left
+// out), and the row's memory becomes the half planes of 2^kF16Exp (softmax -
+// onehot): hi in its first ld halves, lo in the next ld; zeros for rows left out
+// and for the columns from V to ld.
 void xent_rows(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, int64_t row0,
-               float* nll, bool grad);
+               float* nll);
 
-// v[0 .. n) *= 1 / max(1, count[0])
-void scale_by_count(float* v, int64_t n, const int* count);
+// nll[r] of n rows from the statistics of gemm_f16_lse
+void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,
+               float* nll);
 
 // loss[0] = sum of v[0 .. n) / max(1, count[0])
 void loss_mean(const float* v, int64_t n, const int* count, float* loss);

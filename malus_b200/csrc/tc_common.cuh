@@ -334,5 +334,8 @@ __device__ __forceinline__ float tf32_rn(float x) {
 // swizzle is a CUtensorMapSwizzle value.  Defined in gemm.cu.
 CUtensorMap encode_f32_map(int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
                            const uint32_t* box, int swizzle);
+// The same for half values, 128-byte swizzle.
+CUtensorMap encode_f16_map(int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                           const uint32_t* box);
 
 }  // namespace malus
