@@ -11,19 +11,18 @@
 // with products of known sums: a chain of n additions loses about n * 2e-8 of
 // the magnitude, all in one direction; K = 50304 as one chain is off by 8e-5).
 // So a chain is kept short: within a 64-deep stage the small cross products come
-// first, then the four hi*hi additions, and after every second stage (K = 128)
+// first, then the four hi*hi additions, and after every fourth stage (K = 256)
 // the epilogue warps take the accumulator out of tensor memory and add it,
 // rounding to nearest, to sums in their registers, while the tensor core fills
-// the other accumulator.  That costs no tensor time: 128 rows x 256 columns
-// are read in well under the 3072 cycles the next 128 of K take.
+// the other accumulator.
 //
 // Work: 2-CTA clusters, each unit a 256 x 256 tile (one tcgen05.mma of M = 256
 // per k-step, cta_group::2) over all of K or a slice of it.  Each CTA loads its
 // 128 rows of A and 128 of B, both planes, 64 deep: 64 KB a stage, three stages,
 // so an SM takes in 64 KB per 1536 cycles of tensor time.  A single CTA's 128 x
 // 256 tile would take 96 KB per the same time, more than L2 delivers.
-// Warp 0 issues the TMA loads, warp 1 (of rank 0) the MMAs, warps 2-9 hold the
-// sums (a row of 128 columns per thread) and store.
+// Warp 0 issues the TMA loads, warp 1 (of rank 0) the MMAs, warps 4-11 hold the
+// sums (128 columns of a row per thread) and store by TMA.
 #include "gemm_f16.cuh"
 #include "tc_common.cuh"
 
@@ -36,9 +35,16 @@ using namespace malus::tc;
 constexpr int BM = 128, BN = 256, BK = 64, STAGES = 3;
 constexpr int kTile = 128 * BK * 2;                 // one plane's 128 rows, 64 deep
 constexpr int kStageBytes = 4 * kTile;              // A hi, A lo, B hi, B lo
-constexpr int kChunk = 2;                           // stages per accumulator
-constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
-constexpr int kSmem = STAGES * kStageBytes + 1024 + 256;
+constexpr int kChunk = 4;                           // stages per accumulator
+constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
+constexpr int kCols = BN * 4 / kEpiWarps;           // columns of a row that an epilogue thread holds
+// Registers per thread: 168 at launch; the warpgroup of the TMA and MMA warps
+// gives up all but 40, the two epilogue warpgroups take 232 (128 sums, 32 in
+// flight from tensor memory).  128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kRegsLaunch = 168, kRegsIo = 40, kRegsEpi = 232;
+static_assert(128 * kRegsIo + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "registers");
+constexpr int kStaging = 32 * 32 * 4;               // per epilogue warp: 32 rows x 32 columns
+constexpr int kSmem = STAGES * kStageBytes + 1024 + 256 + kEpiWarps * kStaging;
 static_assert(kSmem <= 232448, "shared memory");
 
 struct Params {
@@ -47,9 +53,7 @@ struct Params {
   int64_t a_k0, b_k0;
   const float *a_inv, *b_inv;
   float inv_all;
-  float* out;          // (split, m, n) at split * sstride + m * ldo + n (trans: + n * ldo + m)
-  int64_t ldo, sstride;
-  int trans, accumulate;
+  int accumulate;
   const int* count;
   int inner_m;         // consecutive units walk M (else N)
   float2* part;
@@ -93,82 +97,76 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t tile, bool mn) {
 
 enum Mode : int { kStore = 0, kLse = 1 };
 
-// The 128 sums acc of row m, columns n0 .. n0 + 127, into the output or the row's statistics.
-template <int MODE>
-__device__ __forceinline__ void finish_row(const Params& p, const Unit& un, float (&acc)[128], int m, int n0,
-                                           float alpha) {
+// The sums acc of 32 rows from m0 (one per lane), columns n0 .. n0 + kCols - 1:
+// scaled and sent to the output 32 columns at a time through the warp's staging
+// block, which a TMA store (or, accumulating, a TMA add: one per element and
+// launch, so the order is fixed) takes from there.  The copy drops what lies
+// past M or N.
+__device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap* mOut, const Unit& un,
+                                             float (&acc)[kCols], int m0, int n0, float alpha, uint8_t* stage) {
+  const int lane = threadIdx.x & 31, m = m0 + lane;
+  if (m0 >= p.M) return;   // uniform over the warp
+  const float sa = alpha * (p.a_inv && m < p.M ? p.a_inv[m] : 1.0f);
+  float4* mine = reinterpret_cast<float4*>(stage + lane * 128);
+#pragma unroll
+  for (int c = 0; c < kCols; c += 32) {
+    if (n0 + c >= p.N) break;
+    if (lane == 0) bulk_wait_read<0>();   // the block's last copy has left it
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {   // 16-byte granule g of row r lies at g ^ (r & 7): the map's swizzle
+      float4 v = make_float4(acc[c + 4 * g] * sa, acc[c + 4 * g + 1] * sa, acc[c + 4 * g + 2] * sa,
+                             acc[c + 4 * g + 3] * sa);
+      if (p.b_inv) {   // padded to whole tiles by the host
+        const float4 sb = *reinterpret_cast<const float4*>(p.b_inv + n0 + c + 4 * g);
+        v.x *= sb.x; v.y *= sb.y; v.z *= sb.z; v.w *= sb.w;
+      }
+      mine[g ^ (lane & 7)] = v;
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (p.accumulate) tma_add_3d(mOut, smem_u32(stage), n0 + c, m0, un.split);
+      else tma_store_3d(mOut, smem_u32(stage), n0 + c, m0, un.split);
+      bulk_commit();
+    }
+  }
+}
+
+// The sums of a row into its maximum, sum of exponentials and target value.
+__device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols], int m, int n0, float alpha) {
   if (m >= p.M) return;
   const float sa = alpha * (p.a_inv ? p.a_inv[m] : 1.0f);
-  if (MODE == kLse) {
-    float mx = -INFINITY;
+  float mx = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 128; ++j) {
-      acc[j] = n0 + j < p.N ? acc[j] * sa * p.b_inv[n0 + j] : -INFINITY;
-      mx = fmaxf(mx, acc[j]);
-    }
-    float s = 0.0f;
-    const float mm = mx == -INFINITY ? 0.0f : mx;
-#pragma unroll
-    for (int j = 0; j < 128; ++j) s += exp2f((acc[j] - mm) * kLog2e);
-    p.part[(int64_t)m * (2 * p.tiles_n) + (n0 >> 7)] = make_float2(mx, s);
-    const int64_t t = p.tdt == MALUS_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
-    if (t >= n0 && t < n0 + 128 && t < p.N) {
-      const int o = (int)(t - n0);
-      float zt = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 128; ++j)
-        if (j == o) zt = acc[j];
-      p.at[m] = zt;
-    }
-    return;
+  for (int j = 0; j < kCols; ++j) {
+    acc[j] = n0 + j < p.N ? acc[j] * sa * p.b_inv[n0 + j] : -INFINITY;
+    mx = fmaxf(mx, acc[j]);
   }
-  if (p.trans) {   // lanes are neighbours in m: whole 128-byte lines
-    float* o = p.out + (int64_t)un.split * p.sstride + m;
+  float s = 0.0f;
+  const float mm = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-    for (int j = 0; j < 128; ++j) {
-      const int n = n0 + j;
-      if (n < p.N) {
-        const float v = acc[j] * sa * (p.b_inv ? p.b_inv[n] : 1.0f);
-        float* q = o + (int64_t)n * p.ldo;
-        *q = p.accumulate ? *q + v : v;
-      }
-    }
-    return;
-  }
-  float* o = p.out + (int64_t)un.split * p.sstride + (int64_t)m * p.ldo + n0;
-  const bool vec = ((uintptr_t)o & 15) == 0;
+  for (int j = 0; j < kCols; ++j) s += exp2f((acc[j] - mm) * kLog2e);
+  p.part[(int64_t)m * (BN / kCols * p.tiles_n) + n0 / kCols] = make_float2(mx, s);
+  const int64_t t = p.tdt == MALUS_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
+  if (t >= n0 && t < n0 + kCols && t < p.N) {
+    const int o = (int)(t - n0);
+    float zt = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 128; j += 4) {
-    const int n = n0 + j;
-    if (vec && n + 4 <= p.N) {
-      float4 v = make_float4(acc[j] * sa, acc[j + 1] * sa, acc[j + 2] * sa, acc[j + 3] * sa);
-      if (p.b_inv) {
-        v.x *= p.b_inv[n]; v.y *= p.b_inv[n + 1]; v.z *= p.b_inv[n + 2]; v.w *= p.b_inv[n + 3];
-      }
-      float4* q = reinterpret_cast<float4*>(o + j);
-      if (p.accumulate) {
-        const float4 c = *q;
-        v.x += c.x; v.y += c.y; v.z += c.z; v.w += c.w;
-      }
-      *q = v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < p.N) {
-          const float v = acc[j + i] * sa * (p.b_inv ? p.b_inv[n + i] : 1.0f);
-          o[j + i] = p.accumulate ? o[j + i] + v : v;
-        }
-    }
+    for (int j = 0; j < kCols; ++j)
+      if (j == o) zt = acc[j];
+    p.at[m] = zt;
   }
 }
 
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUtensorMap mAl,
-           const __grid_constant__ CUtensorMap mBh, const __grid_constant__ CUtensorMap mBl, const Params p) {
+           const __grid_constant__ CUtensorMap mBh, const __grid_constant__ CUtensorMap mBl,
+           const __grid_constant__ CUtensorMap mOut, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = (uint64_t*)(smem + STAGES * kStageBytes);
+  uint64_t* full = (uint64_t*)(smem + STAGES * kStageBytes + kEpiWarps * kStaging);
   uint64_t* empty = full + STAGES;
   uint64_t* accf = empty + STAGES;
   uint64_t* acce = accf + 2;
@@ -208,6 +206,8 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIo));
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
@@ -301,18 +301,21 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
       }
       if (!ok) *abort_flag = 1;
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     // ---------------- epilogue ----------------
-    // Warp w owns lane quarter w % 4 (32 rows, one per lane) and 128 of the
+    // Warp w owns lane quarter w % 4 (32 rows, one per lane) and kCols of the
     // tile's columns.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * kCols);
+    uint8_t* stage = smem + STAGES * kStageBytes + (warp - 4) * kStaging;
     const float alpha = p.inv_all * (p.count ? 1.0f / (float)max(1, *p.count) : 1.0f);
     uint32_t chunk = 0;
     bool ok = true;
     for (int u = grp; u < total && ok; u += ngrp) {
       const Unit un = unit_at(p, u);
-      float acc[128];
+      float acc[kCols];
       for (int st = un.st_lo; st < un.st_hi; st += kChunk, ++chunk) {
         const uint32_t b = chunk & 1;
         if (!mbar_wait(smem_u32(&accf[b]), (chunk >> 1) & 1, abort_flag, p.err, 43)) {
@@ -322,14 +325,14 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (st == un.st_lo) {
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) tmem_ld16(tbase + b * BN + c, reinterpret_cast<uint32_t*>(acc + c));
+          for (int c = 0; c < kCols; c += 32) tmem_ld32(tbase + b * BN + c, reinterpret_cast<uint32_t*>(acc + c));
         } else {
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) {   // 16 at a time: the sums leave no registers for more
-            uint32_t r[16];
-            tmem_ld16(tbase + b * BN + c, r);
+          for (int c = 0; c < kCols; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(tbase + b * BN + c, r);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(r[j]);
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -337,9 +340,12 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
         if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acce[b]), 0));
       }
       if (!ok) break;
-      finish_row<MODE>(p, un, acc, un.m0 + (int)rank * BM + quarter * 32 + lane, un.n0 + half * 128, alpha);
+      const int m0 = un.m0 + (int)rank * BM + quarter * 32, n0 = un.n0 + part * kCols;
+      if (MODE == kLse) finish_lse(p, acc, m0 + lane, n0, alpha);
+      else finish_store(p, &mOut, un, acc, m0, n0, alpha, stage);
       __syncwarp();   // rows past M return early: the next tensor memory load needs the whole warp
     }
+    if (MODE == kStore && lane == 0) bulk_wait<0>();   // every copy is done before the CTA exits
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(done));
@@ -357,18 +363,34 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
   }
 }
 
-// out = sum over the K slices, in slice order, of ws[s][m][n] (row pitch ldw)
-__global__ void k_f16_join(const float* __restrict__ ws, int splits, int64_t sstride, int M, int N, int64_t ldw,
-                           float* __restrict__ out, int64_t ldo, int trans, int accumulate) {
-  const int64_t total = (int64_t)M * N;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = trans ? i % M : i / N, n = trans ? i / M : i % N;
-    float s = 0.0f;
+// out = sum over the K slices, in slice order, of ws[s][m][n] (row pitch ldw, a
+// multiple of 4); a block takes 1024 columns of a row
+template <bool VEC>
+__global__ void __launch_bounds__(256) k_f16_join(const float* __restrict__ ws, int splits, int64_t sstride, int N,
+                                                  int64_t ldw, float* __restrict__ out, int64_t ldo, int accumulate) {
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= N) return;
+  const float* p = ws + (int64_t)blockIdx.y * ldw + n;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += ws[k * sstride + m * ldw + n];
-    float* o = out + (trans ? n * ldo + m : m * ldo + n);
-    *o = accumulate ? *o + s : s;
+  for (int k = 0; k < splits; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(p + k * sstride);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
+  float* o = out + (int64_t)blockIdx.y * ldo + n;
+  if (VEC && n + 4 <= N) {
+    float4* q = reinterpret_cast<float4*>(o);
+    if (accumulate) {
+      const float4 w = *q;
+      s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+    }
+    *q = s;
+    return;
+  }
+  const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < N) o[i] = accumulate ? o[i] + x[i] : x[i];
 }
 
 // ------------------------------------------------------------------ planes
@@ -514,6 +536,10 @@ cudaLaunchConfig_t config(int grid, cudaLaunchAttribute* at) {
   static bool attr = false;
   if (!attr) {
     MALUS_CUDA(cudaFuncSetAttribute(k_gemm_f16<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    // the register split draws on what the launch reserves: fewer would wait forever
+    cudaFuncAttributes fa;
+    MALUS_CUDA(cudaFuncGetAttributes(&fa, k_gemm_f16<MODE>));
+    if (fa.numRegs < kRegsLaunch) panic("gemm_f16: %d registers per thread at launch, %d needed", fa.numRegs, kRegsLaunch);
     attr = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -543,8 +569,10 @@ int max_pairs() {
   return n;
 }
 
+// out: [splits][M][N], rows ldo floats apart (a multiple of 4, 16-byte aligned
+// base), slices sstride; null in kLse mode.
 template <int MODE>
-void launch(const F16Gemm& g, Params& p) {
+void launch(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstride) {
   p.M = g.M; p.N = g.N; p.K = g.K;
   p.tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (g.N + BN - 1) / BN;
@@ -557,10 +585,17 @@ void launch(const F16Gemm& g, Params& p) {
   const int units = p.tiles_m * p.tiles_n * p.splits;
   cudaLaunchAttribute at[1];
   cudaLaunchConfig_t cfg = config<MODE>(2 * std::min(units, max_pairs()), at);
+  CUtensorMap mo = {};
+  if (MODE == kStore) {
+    const uint64_t dims[3] = {(uint64_t)g.N, (uint64_t)g.M, (uint64_t)p.splits};
+    const uint64_t st[2] = {(uint64_t)ldo * 4, (uint64_t)sstride * 4};
+    const uint32_t box[3] = {32, 32, 1};
+    mo = encode_f32_map(3, out, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
   const int pid = prof_begin(0, 2.0 * g.M * (double)g.N * g.K,
                              4.0 * ((double)g.M * g.K + (double)g.N * g.K) + 4.0 * (double)g.M * g.N);
   MALUS_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_f16<MODE>, map_of(g.a, g.a.hi), map_of(g.a, g.a.lo), map_of(g.b, g.b.hi),
-                                map_of(g.b, g.b.lo), p));
+                                map_of(g.b, g.b.lo), mo, p));
   count_launch();
   after_launch("k_gemm_f16");
   prof_end(pid);
@@ -590,26 +625,30 @@ void gemm_f16(const F16Gemm& g) {
   const int tiles = ((g.M + 2 * BM - 1) / (2 * BM)) * ((g.N + BN - 1) / BN);
   p.splits = splits_for(tiles, p.nst, max_pairs());
   p.count = g.count;
-  if (p.splits == 1) {
-    p.out = g.out;
-    p.ldo = g.ldo;
-    p.trans = g.trans;
+  if (p.splits == 1 && g.ldo % 4 == 0 && ((uintptr_t)g.out & 15) == 0) {
     p.accumulate = g.accumulate;
-    launch<kStore>(g, p);
+    launch<kStore>(g, p, g.out, g.ldo, (int64_t)g.M * g.ldo);
     return;
   }
-  p.ldo = (g.N + 3) / 4 * 4;
-  p.sstride = (int64_t)g.M * p.ldo;
-  p.out = static_cast<float*>(scratch_alloc((size_t)p.sstride * p.splits * 4));
-  launch<kStore>(g, p);
-  k_f16_join<<<grid_for((size_t)g.M * g.N, 256), 256, 0, stream()>>>(p.out, p.splits, p.sstride, g.M, g.N, p.ldo, g.out,
-                                                                     g.ldo, g.trans, g.accumulate);
-  count_launch();
+  // K slices, or rows that a TMA store cannot address: through a workspace
+  const int64_t ldw = ((int64_t)g.N + 3) / 4 * 4, sstride = (int64_t)g.M * ldw;
+  float* ws = static_cast<float*>(scratch_alloc((size_t)sstride * p.splits * 4));
+  launch<kStore>(g, p, ws, ldw, sstride);
+  const unsigned gx = (unsigned)((g.N + 1023) / 1024);
+  for (int m0 = 0; m0 < g.M; m0 += 65535) {
+    const dim3 grid(gx, (unsigned)std::min(65535, g.M - m0));
+    float* o = g.out + (int64_t)m0 * g.ldo;
+    const float* w = ws + (int64_t)m0 * ldw;
+    if (g.ldo % 4 == 0 && ((uintptr_t)g.out & 15) == 0)
+      k_f16_join<true><<<grid, 256, 0, stream()>>>(w, p.splits, sstride, g.N, ldw, o, g.ldo, g.accumulate);
+    else k_f16_join<false><<<grid, 256, 0, stream()>>>(w, p.splits, sstride, g.N, ldw, o, g.ldo, g.accumulate);
+    count_launch();
+  }
   after_launch("k_f16_join");
-  scratch_free(p.out);
+  scratch_free(ws);
 }
 
-int f16_lse_parts(int N) { return 2 * ((N + BN - 1) / BN); }
+int f16_lse_parts(int N) { return BN / kCols * ((N + BN - 1) / BN); }
 
 void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target, int tgt_dtype) {
   if (g.M <= 0) return;
@@ -620,7 +659,7 @@ void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target,
   p.at = at;
   p.target = target;
   p.tdt = tgt_dtype;
-  launch<kLse>(g, p);
+  launch<kLse>(g, p, nullptr, 0, 0);
 }
 
 void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv) {

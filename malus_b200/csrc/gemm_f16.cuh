@@ -20,14 +20,15 @@ struct F16Operand {
   float inv_all;
 };
 
-// out[m * ldo + n] (or out[n * ldo + m] with trans) = A B^T / max(1, count[0])
-// (count null: as it is), added to what is there with accumulate.
+// out[m * ldo + n] = A B^T / max(1, count[0]) (count null: as it is), added to
+// what is there with accumulate.  A B operand with per-row scales has them
+// padded to whole tiles of 256 (f16_scales).
 struct F16Gemm {
   int M, N, K;
   F16Operand a, b;
   float* out;
   int64_t ldo;
-  bool trans, accumulate;
+  bool accumulate;
   const int* count;
 };
 void gemm_f16(const F16Gemm& g);
@@ -48,6 +49,9 @@ void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* 
 void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
                     int keep_dtype, int64_t limit);
 inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+
+// floats behind the scales of `rows` plane rows: a GEMM reads whole tiles of them
+inline int64_t f16_scales(int64_t rows) { return (rows + 255) / 256 * 256; }
 
 constexpr int kF16Exp = 13;   // scaled magnitudes stay below 2^(kF16Exp + 1)
 

@@ -32,7 +32,7 @@ struct Planes {
   int64_t rows, pitch;
   Planes(int64_t r, int64_t cols) : rows(r), pitch(pad64(cols)) {
     const size_t plane = (size_t)rows * pitch;
-    hi = static_cast<__half*>(scratch_alloc(plane * 4 + (size_t)rows * 4));
+    hi = static_cast<__half*>(scratch_alloc(plane * 4 + (size_t)f16_scales(rows) * 4));
     lo = hi + plane;
     inv = reinterpret_cast<float*>(lo + plane);
   }
@@ -61,16 +61,18 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   constexpr float inv = 1.0f / (1 << kF16Exp);
   for (int64_t r0 = 0; r0 < n; r0 += piece) {
     const int64_t m = std::min(piece, n - r0);
-    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), logits, ld, false, false, nullptr};
+    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), logits, ld, false, nullptr};
     gemm_f16(g);
     xent_rows(logits, ld, m, V, tgt, tdt, r0, nll);
     if (dx) {
       const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, false, 0, nullptr, inv};
-      gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, false, count});
+      gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, count});
     }
     if (dw) {
       const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, true, 0, nullptr, inv};
-      gemm_f16({(int)V, (int)D, (int)m, dl, xc.kmajor(0, D, r0), dw, tied ? D : V, !tied, r0 > 0, count});
+      const F16Operand xt = xc.kmajor(0, D, r0);
+      if (tied) gemm_f16({(int)V, (int)D, (int)m, dl, xt, dw, D, r0 > 0, count});
+      else gemm_f16({(int)D, (int)V, (int)m, xt, dl, dw, V, r0 > 0, count});
     }
   }
   scratch_free(logits);
@@ -85,7 +87,7 @@ void loss_only(const void* tgt, int tdt, int64_t n, int64_t D, int64_t V, const 
   for (int64_t r0 = 0; r0 < n; r0 += piece) {
     const int64_t m = std::min(piece, n - r0);
     const void* t = static_cast<const char*>(tgt) + r0 * (int64_t)dtype_size(tdt);
-    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), nullptr, 0, false, false, nullptr};
+    F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), nullptr, 0, false, nullptr};
     gemm_f16_lse(g, part, at, t, tdt);
     xent_join(part, parts, at, t, tdt, V, m, nll + r0);
   }

@@ -8,9 +8,9 @@ term is within 1.5 * 2^-22 of itself (two operand roundings and the dropped
 product of the low parts), plus 2^-39 of the row's largest element for elements
 far below it.  The tensor core truncates: an addition into its accumulator loses
 up to 2^-23 of the partial sum, and aligning the 16 products of an instruction
-as much again; a chain holds 24 instructions (128 of K) before it is added, rounding
+as much again; a chain holds 48 instructions (256 of K) before it is added, rounding
 to nearest (2^-24), to the others.  With A = sum |a_k b_k| that bounds the error
-by (3 + 48 + K / 256) 2^-23 A.  The softmax itself is within (80 + 4 |z|) 2^-24
+by (3 + 96 + K / 512) 2^-23 A.  The softmax itself is within (80 + 4 |z|) 2^-24
 relative (as in the distillation tests)."""
 import ctypes as C
 
@@ -23,7 +23,7 @@ U = 2.0 ** -24
 
 def prod_tol(absa, absb, K):
     """error bound of A B^T for |A| [m, K], |B| [n, K]"""
-    t = (52 + K / 256) * 2.0 ** -23 * (absa @ absb.T)
+    t = (99 + K / 512) * 2.0 ** -23 * (absa @ absb.T)
     t += 2.0 ** -39 * (absa.max(1, initial=0)[:, None] * absb.sum(1)[None] + absa.sum(1)[:, None] * absb.max(1, initial=0)[None])
     return t
 
