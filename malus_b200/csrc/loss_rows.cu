@@ -4,14 +4,21 @@
 //   p = softmax over the row's entries of teacher / T,  q = softmax(logits / T)
 //   kl = T^2 sum_k p_k (log p_k - log q[id_k]),  dlogits = T (q - p) / rows
 //
-// Bound by HBM: a row is read once and held in registers, by one block or by a
-// cluster of up to 8 that exchange their maximum and sum through distributed
-// shared memory, so the gradient row is written without reading the logits
-// again (4 B read and 4 B written per logit).
+// Bound by HBM: a row is read once and held in registers, so its gradient is
+// written without reading the logits again (4 B read and 4 B written per logit).
+// Rows up to 1024 logits take a warp each.  Longer ones take a block, or a
+// cluster of up to 8 blocks that exchange their maximum and sum through
+// distributed shared memory.  The blocks stay and walk the rows: while a row is
+// in registers (maximum, exponentials, exchange, gradient), the bulk copy of the
+// next one is already landing in shared memory, which keeps reads in flight
+// through the phases that wait.
 #include "gemm_f16.cuh"
 #include "loss_rows.cuh"
+#include "tc_common.cuh"
 
 #include <cooperative_groups.h>
+#include <mutex>
+#include <map>
 
 namespace cg = cooperative_groups;
 
@@ -19,10 +26,12 @@ namespace malus {
 namespace {
 
 constexpr int kNV = 8;            // float4 groups a thread holds
-constexpr int kThreads = 512;     // usual most per block; twice that for the longest rows
-constexpr int kMaxThreads = 1024;
+constexpr int kThreads = 448;     // most per block: two blocks per SM with 72 registers each
+constexpr int kMaxThreads = 1024; // for rows that eight such blocks do not hold
 constexpr int kMaxCluster = 8;
 constexpr int kMaxEntries = 1024; // teacher entries of a row
+constexpr int kShort = 32 * kNV * 4 - 4;   // longest row of a warp (it may start 3 past a 16-byte group)
+constexpr int kWarps = 8;         // rows per block of the short-row kernels
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kErrId = 4;         // the error word's code for an id out of range
 
@@ -40,102 +49,162 @@ __device__ __forceinline__ float wsum(float v) {
   return v;
 }
 
-// A row of V floats at `row` as 16-byte groups from the aligned address at or
-// below it: group i covers elements 4 i - shift .. 4 i - shift + 3, and the
-// groups that reach past either end of the row are read and written by element.
+// A row of V floats as 16-byte groups from the aligned address at or below it:
+// group i covers elements 4 i - shift .. 4 i - shift + 3.  Groups [w0, w1) lie
+// wholly in the row; the one before or after them reaches past its end and is read
+// and written by element.
 struct RowSlice {
-  int shift;        // elements between the aligned address and the row
-  int64_t g0, g1;   // this block's groups
+  const float4* base;   // group 0
+  int shift;            // elements between the aligned address and the row
+  int g0, g1;           // this block's groups
+  int w0, w1;
 };
-__device__ __forceinline__ RowSlice slice_of(const float* row, int64_t V, int rank, int cs) {
+__device__ __forceinline__ RowSlice slice_of(const float* row, int V, int rank, int cs) {
   RowSlice s;
   s.shift = (int)(((uintptr_t)row >> 2) & 3);
-  const int64_t groups = (V + s.shift + 3) / 4, per = (groups + cs - 1) / cs;
-  s.g0 = rank * per;
-  s.g1 = s.g0 + per < groups ? s.g0 + per : groups;
+  s.base = reinterpret_cast<const float4*>(row - s.shift);
+  const int groups = (V + s.shift + 3) / 4, per = (groups + cs - 1) / cs;
+  s.g0 = min(rank * per, groups);
+  s.g1 = min(s.g0 + per, groups);
+  s.w0 = s.shift ? 1 : 0;
+  s.w1 = (V + s.shift) / 4;
   return s;
 }
-__device__ __forceinline__ float4 load_group(const float* __restrict__ row, int64_t V, int64_t e) {
-  if (e >= 0 && e + 4 <= V) return *reinterpret_cast<const float4*>(row + e);
-  float4 q;
+__device__ __forceinline__ float4 load_edge(const float* __restrict__ row, int V, int e) {
   const float ninf = -INFINITY;
-  q.x = e >= 0 && e < V ? row[e] : ninf;
-  q.y = e + 1 >= 0 && e + 1 < V ? row[e + 1] : ninf;
-  q.z = e + 2 >= 0 && e + 2 < V ? row[e + 2] : ninf;
-  q.w = e + 3 >= 0 && e + 3 < V ? row[e + 3] : ninf;
-  return q;
+  return make_float4(e >= 0 && e < V ? row[e] : ninf, e + 1 >= 0 && e + 1 < V ? row[e + 1] : ninf,
+                     e + 2 >= 0 && e + 2 < V ? row[e + 2] : ninf, e + 3 >= 0 && e + 3 < V ? row[e + 3] : ninf);
 }
-__device__ __forceinline__ void store_group(float* __restrict__ row, int64_t V, int64_t e, float4 q, bool vec) {
-  if (vec && e >= 0 && e + 4 <= V) {
-    *reinterpret_cast<float4*>(row + e) = q;
-    return;
-  }
+__device__ __forceinline__ void store_edge(float* __restrict__ row, int V, int e, float4 q) {
   if (e >= 0 && e < V) row[e] = q.x;
   if (e + 1 >= 0 && e + 1 < V) row[e + 1] = q.y;
   if (e + 2 >= 0 && e + 2 < V) row[e + 2] = q.z;
   if (e + 3 >= 0 && e + 3 < V) row[e + 3] = q.w;
 }
 
-// Maximum and sum of exponentials of the row whose groups the cluster's threads
-// hold in v: v becomes exp((v - max) * c), and the sum is over the whole row.
-// Elements of -inf give 0; a row of -inf only, or with a +inf or NaN, gives NaN
-// probabilities as the formula does.  Every block has read its slice when this
-// returns.
+// Maximum and sum of exponentials of a row whose groups the threads hold in v
+// (n of them in this thread): v becomes exp((v - max) * c) after row_scale, and
+// the sum is over the whole row.  Elements of -inf give 0; a row of -inf only, or
+// with a +inf or NaN, gives NaN probabilities as the formula does.
 struct RowStat { float max, sum; };
-__device__ __forceinline__ RowStat row_stat(float4 (&v)[kNV], int n, float c, cg::cluster_group& cl, float* red,
-                                            float2* mine) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+
+// The warp's maximum; v becomes exp against it and the sum is the warp's.  The
+// exponential is the hardware's base-2 one (relative error 2^-22; results
+// below 2^-126 are 0).
+__device__ __forceinline__ RowStat warp_stat(float4 (&v)[kNV], int n, float c) {
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kNV; ++k)
     if (k < n) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
   m = wmax(m);
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-  m = -INFINITY;
-  for (int i = 0; i < warps; ++i) m = fmaxf(m, red[i]);
-  // exponentials against the block's own maximum; the blocks are joined below
   const float m0 = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
 #pragma unroll
   for (int k = 0; k < kNV; ++k)
     if (k < n) {
-      v[k].x = exp2f((v[k].x - m0) * c);
-      v[k].y = exp2f((v[k].y - m0) * c);
-      v[k].z = exp2f((v[k].z - m0) * c);
-      v[k].w = exp2f((v[k].w - m0) * c);
+      v[k].x = tc::exp2_hw((v[k].x - m0) * c);
+      v[k].y = tc::exp2_hw((v[k].y - m0) * c);
+      v[k].z = tc::exp2_hw((v[k].z - m0) * c);
+      v[k].w = tc::exp2_hw((v[k].w - m0) * c);
       s += (v[k].x + v[k].y) + (v[k].z + v[k].w);
     }
-  s = wsum(s);
-  if (lane == 0) red[32 + warp] = s;
-  __syncthreads();
-  s = 0.0f;
-  for (int i = 0; i < warps; ++i) s += red[32 + i];
-  const int cs = (int)cl.num_blocks();
-  if (cs == 1) return {m, s};
-  if (threadIdx.x == 0) *mine = make_float2(m, s);
-  cl.sync();
-  float M = -INFINITY;
-  for (int r = 0; r < cs; ++r) M = fmaxf(M, cl.map_shared_rank(mine, r)->x);
-  // a block of -inf only has the sum 0 (or NaN) whatever its factor
-  auto factor = [&](float bm) { return bm == -INFINITY ? 1.0f : exp2f((bm - M) * c); };
-  float S = 0.0f;
-  for (int r = 0; r < cs; ++r) {
-    const float2 o = *cl.map_shared_rank(mine, r);
-    S += o.y * factor(o.x);
-  }
-  const float f = factor(m);
-#pragma unroll
-  for (int k = 0; k < kNV; ++k)
-    if (k < n) v[k] = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
-  cl.sync();   // no block leaves while another still reads its pair
-  return {M, S};
+  return {m, wsum(s)};
 }
+// a part of -inf only has the sum 0 (or NaN) whatever its factor
+__device__ __forceinline__ float join_factor(float m, float M, float c) {
+  return m == -INFINITY ? 1.0f : tc::exp2_hw((m - M) * c);
+}
+
+// Joins the warps of a cluster of blocks (or of one block): every warp writes its
+// pair into each block's table, one barrier, and every warp reduces the table.
+// `f` is what brings this warp's exponentials to the row's maximum.  Two tables
+// alternate: with one cluster barrier per row nobody overwrites one that another
+// warp may still read.  Every block has its slice in registers when this returns.
+__device__ __forceinline__ RowStat join(RowStat w, float c, cg::cluster_group& cl, float2* table, float* f) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int cs = (int)cl.num_blocks(), total = cs * warps;
+  if (cs == 1) {
+    if (lane == 0) table[warp] = make_float2(w.max, w.sum);
+    __syncthreads();
+  } else {
+    if (lane < cs) *cl.map_shared_rank(table + cl.block_rank() * warps + warp, lane) = make_float2(w.max, w.sum);
+    cl.sync();
+  }
+  float M = -INFINITY;
+  for (int i = lane; i < total; i += 32) M = fmaxf(M, table[i].x);
+  M = wmax(M);
+  float S = 0.0f;
+  for (int i = lane; i < total; i += 32) S += table[i].y * join_factor(table[i].x, M, c);
+  *f = join_factor(w.max, M, c);
+  return {M, wsum(S)};
+}
+constexpr int kTable = kMaxCluster * kMaxThreads / 32;
+
+// The landing buffer: the slice of the next row, brought by a bulk copy of its
+// whole 16-byte groups (the groups that reach past the row are read from memory
+// by the thread that holds them).  A copy that does not arrive within the wait's
+// bound is reported in the error word; no further copy is then issued or waited for.
+struct Landing {
+  float4* buf;
+  uint32_t bar;
+  uint32_t parity;
+  bool dead;
+  int32_t* err;
+
+  __device__ __forceinline__ void init(float4* b, uint64_t* mbar, int32_t* e) {
+    buf = b;
+    bar = tc::smem_u32(mbar);
+    parity = 0;
+    dead = false;
+    err = e;
+    if (threadIdx.x == 0) {
+      tc::mbar_init(bar, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ void issue(const RowSlice& s) {
+    if (threadIdx.x != 0 || dead) return;
+    const int i0 = max(s.g0, s.w0), i1 = min(s.g1, s.w1);
+    const uint32_t bytes = i1 > i0 ? (uint32_t)(i1 - i0) * 16 : 0;
+    tc::mbar_expect_tx(bar, bytes);
+    if (bytes)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(tc::smem_u32(buf + (i0 - s.g0))), "l"(s.base + i0), "r"(bytes), "r"(bar)
+                   : "memory");
+  }
+  __device__ __forceinline__ void wait() {
+    if (dead) return;
+    if (!tc::mbar_try(bar, parity)) {
+      const uint64_t t0 = tc::gtimer();
+      while (!tc::mbar_try(bar, parity))
+        if (tc::gtimer() - t0 > tc::kWaitNs) {
+          dead = true;
+          atomicExch(err, 51);
+          break;
+        }
+    }
+    parity ^= 1;
+  }
+  // whether this thread holds group g of the slice
+  __device__ __forceinline__ bool holds(const RowSlice& s, int g) const {
+    return g >= s.g0 && g < s.g1 && (g - s.g0) % (int)blockDim.x == (int)threadIdx.x;
+  }
+  // this thread's groups of the landed slice into v; returns how many
+  __device__ __forceinline__ int take(float4 (&v)[kNV], const RowSlice& s) const {
+    const int len = s.g1 - s.g0, nt = (int)blockDim.x, t = (int)threadIdx.x;
+    const int n = len > t ? (len - t + nt - 1) / nt : 0;
+#pragma unroll
+    for (int k = 0; k < kNV; ++k)
+      if (k < n) v[k] = buf[t + k * nt];
+    return n;
+  }
+};
 
 // Four elements of the row's gradient, magnitudes at most 1, as the half planes
 // that the head's products read: hi in the first half of the row's memory, lo in
 // the second.
-__device__ __forceinline__ void store_planes(float* row, int64_t ld, int64_t e, float4 q) {
+__device__ __forceinline__ void store_planes(float* row, int ld, int e, float4 q) {
   constexpr float up = (float)(1 << kF16Exp);
   const float x[4] = {q.x * up, q.y * up, q.z * up, q.w * up};
   __align__(8) __half h[4], l[4];
@@ -149,52 +218,105 @@ __device__ __forceinline__ void store_planes(float* row, int64_t ld, int64_t e, 
   *reinterpret_cast<uint2*>(p + ld + e) = *reinterpret_cast<uint2*>(l);
 }
 
-__global__ void __launch_bounds__(kMaxThreads)
-k_xent_rows(float* __restrict__ logits, int64_t ld, int64_t V, const void* __restrict__ tgt, int tdt, int64_t row0,
-            float* __restrict__ nll) {
-  __shared__ float red[64];
-  __shared__ float2 mine;
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  const int64_t r = blockIdx.x / cs;
-  float* row = logits + r * ld;
-  const RowSlice sl = slice_of(row, ld, rank, cs);   // the pitch is whole groups
-  const int64_t t = id_at(tgt, tdt, row0 + r);
-  const bool counted = t >= 0 && t < V;
-  float zt = 0.0f;
-  if (counted) {
-    if (rank == 0 && threadIdx.x == 0) zt = row[t];
+// the gradient of a row's groups that this thread holds in v (exponentials):
+// group g + k * step
+__device__ __forceinline__ void xent_store(float* row, int ld, const float4 (&v)[kNV], int n, int g, int step,
+                                           float f, int t) {
+#pragma unroll
+  for (int k = 0; k < kNV; ++k)
+    if (k < n) {
+      const int e = 4 * (g + k * step);
+      float4 q = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
+      const unsigned o = (unsigned)(t - e);
+      if (o < 4) {
+        if (o == 0) q.x -= 1.0f;
+        if (o == 1) q.y -= 1.0f;
+        if (o == 2) q.z -= 1.0f;
+        if (o == 3) q.w -= 1.0f;
+      }
+      store_planes(row, ld, e, q);   // columns from V on hold exp(-inf) = 0
+    }
+}
+// Group g (of a row whose memory goes on to its pitch) with -inf from column V on.
+__device__ __forceinline__ float4 cut_group(float4 q, int e, int V) {
+  const float ninf = -INFINITY;
+  return make_float4(e < V ? q.x : ninf, e + 1 < V ? q.y : ninf, e + 2 < V ? q.z : ninf, e + 3 < V ? q.w : ninf);
+}
+
+__global__ void __launch_bounds__(32 * kWarps)
+k_xent_rows_warp(float* __restrict__ logits, int ld, int64_t rows, int V, const void* __restrict__ tgt, int tdt,
+                 int64_t row0, float* __restrict__ nll) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * kWarps) {
+    float* row = logits + r * ld;
+    const int64_t t = id_at(tgt, tdt, row0 + r);
+    if (t < 0 || t >= V) {
+      if (lane == 0) nll[row0 + r] = 0.0f;
+      for (int g = lane; g < ld / 4; g += 32) store_planes(row, ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      continue;
+    }
+    const float zt = row[t];
     float4 v[kNV];
     int n = 0;
 #pragma unroll
     for (int k = 0; k < kNV; ++k) {
-      const int64_t g = sl.g0 + (int64_t)k * blockDim.x + threadIdx.x;
-      if (g < sl.g1) {
-        v[k] = load_group(row, V, 4 * g);
+      const int g = k * 32 + lane;
+      if (g < ld / 4) {
+        v[k] = cut_group(reinterpret_cast<const float4*>(row)[g], 4 * g, V);
         n = k + 1;
       }
     }
-    const RowStat st = row_stat(v, n, kLog2e, cl, red, &mine);
-    if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
-    const float inv = 1.0f / st.sum;
-#pragma unroll
-    for (int k = 0; k < kNV; ++k)
-      if (k < n) {
-        const int64_t e = 4 * (sl.g0 + (int64_t)k * blockDim.x + threadIdx.x);
-        float4 q = make_float4(v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv);
-        if (t >= e && t < e + 4) {
-          if (t == e) q.x -= 1.0f;
-          if (t == e + 1) q.y -= 1.0f;
-          if (t == e + 2) q.z -= 1.0f;
-          if (t == e + 3) q.w -= 1.0f;
-        }
-        store_planes(row, ld, e, q);   // columns from V on hold exp(-inf) = 0
-      }
-  } else {
-    if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = 0.0f;
-    for (int64_t g = sl.g0 + threadIdx.x; g < sl.g1; g += blockDim.x)
-      store_planes(row, ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+    const RowStat st = warp_stat(v, n, kLog2e);   // the whole row is in registers after it
+    if (lane == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
+    xent_store(row, ld, v, n, lane, 32, 1.0f / st.sum, (int)t);
   }
+}
+
+template <int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2)
+k_xent_rows(float* __restrict__ logits, int ld, int64_t rows, int V, const void* __restrict__ tgt, int tdt,
+            int64_t row0, float* __restrict__ nll, int32_t* __restrict__ err) {
+  extern __shared__ __align__(16) float4 land[];
+  __shared__ float2 table[2][kTable];
+  __shared__ uint64_t bar;
+  cg::cluster_group cl = cg::this_cluster();
+  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int64_t step = gridDim.x / cs;
+  Landing L;
+  L.init(land, &bar, err);
+  int64_t r = blockIdx.x / cs;
+  RowSlice sl = slice_of(logits + r * ld, ld, rank, cs);   // the pitch is whole groups: the same in every row
+  if (r < rows) L.issue(sl);
+  int turn = 0;
+  for (; r < rows; r += step) {
+    float* row = logits + r * ld;
+    const int64_t t = id_at(tgt, tdt, row0 + r);
+    const bool counted = t >= 0 && t < V;
+    float zt = 0.0f;
+    if (counted && rank == 0 && threadIdx.x == 0) zt = row[t];
+    L.wait();
+    for (int g = V / 4; g < sl.g1; ++g)   // what lies behind the row is no logit (at most 16 groups)
+      if (L.holds(sl, g)) land[g - sl.g0] = cut_group(land[g - sl.g0], 4 * g, V);
+    float4 v[kNV];
+    const int n = L.take(v, sl);
+    __syncthreads();   // the buffer is free
+    sl.base += step * (ld / 4);
+    if (r + step < rows) L.issue(sl);
+    const int g = sl.g0 + (int)threadIdx.x;
+    if (counted) {
+      float f;
+      const RowStat st = join(warp_stat(v, n, kLog2e), kLog2e, cl, table[turn], &f);
+      turn ^= 1;
+      if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
+      xent_store(row, ld, v, n, g, blockDim.x, f / st.sum, (int)t);
+    } else {
+      if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kNV; ++k)
+        if (k < n) store_planes(row, ld, 4 * (g + k * (int)blockDim.x), make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+  }
+  if (cs > 1) cl.sync();   // no block leaves while another may write its table
 }
 
 __global__ void __launch_bounds__(1024) k_xent_count(const void* __restrict__ tgt, int tdt, int64_t n, int64_t V,
@@ -219,11 +341,19 @@ __global__ void __launch_bounds__(1024) k_xent_count(const void* __restrict__ tg
   }
 }
 
-__global__ void __launch_bounds__(1024) k_loss_mean(const float* __restrict__ v, int64_t n,
-                                                    const int* __restrict__ count, float* __restrict__ loss) {
+// loss = sum of v / max(1, count); with parts, v[r] is first the sum of the row's parts
+__global__ void __launch_bounds__(1024) k_loss_mean(float* __restrict__ v, const float* __restrict__ part, int parts,
+                                                    int64_t n, const int* __restrict__ count, float* __restrict__ loss) {
   __shared__ double sh[32];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += (double)v[i];
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    if (parts) {
+      float a = 0.0f;
+      for (int j = 0; j < parts; ++j) a += part[i * parts + j];
+      v[i] = a;
+    }
+    s += (double)v[i];
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
@@ -266,141 +396,241 @@ __device__ __forceinline__ bool entry_there(int64_t id, float te, int64_t V) {
   return id >= 0 && id < V && te != -INFINITY;
 }
 
-// count[0] += rows with an entry (whole numbers: the order does not matter)
-__global__ void __launch_bounds__(256) k_distill_count(const void* __restrict__ ids, int idt,
-                                                       const float* __restrict__ teacher, int64_t n, int K, int64_t V,
-                                                       int* __restrict__ count, int32_t* __restrict__ err) {
+// An entry of a row: its id (-1: none), p and log p, and for the first entry with
+// this id the p of all of them, -1 for the others.
+struct __align__(16) Entry {
+  int id;
+  float p, lp, own;
+};
+
+// The teacher's side, a warp per row.  flag[r]: the row has an entry; count[0] +=
+// such rows (whole numbers: the order does not matter).
+__global__ void __launch_bounds__(256)
+k_teacher(const void* __restrict__ ids, int idt, const float* __restrict__ teacher, int64_t n, int K, int64_t V,
+          float c, Entry* __restrict__ ent, int* __restrict__ flag, int* __restrict__ count,
+          int32_t* __restrict__ err) {
+  extern __shared__ int sid[];   // [8][K]: the rows' ids, -1 where there is no entry
   __shared__ int sh[8];
   const int lane = threadIdx.x & 31;
-  int c = 0;
+  int* mine = sid + (threadIdx.x >> 5) * K;
+  int rows = 0;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += (int64_t)gridDim.x * 8) {
+    const int64_t o = r * K;
+    float m = -INFINITY;
     bool any = false, bad = false;
     for (int k = lane; k < K; k += 32) {
-      const int64_t id = id_at(ids, idt, r * K + k);
-      any |= entry_there(id, teacher[r * K + k], V);
+      const int64_t id = id_at(ids, idt, o + k);
+      const float te = teacher[o + k];
       bad |= id >= V;
+      const bool there = entry_there(id, te, V);
+      mine[k] = there ? (int)id : -1;
+      if (there) {
+        m = fmaxf(m, te);
+        any = true;
+      }
     }
     if (bad) atomicExch(err, kErrId);
-    c += __any_sync(0xffffffffu, any) ? 1 : 0;
+    m = wmax(m);
+    any = __any_sync(0xffffffffu, any);
+    float s = 0.0f;
+    for (int k = lane; k < K; k += 32) {
+      const float z = (teacher[o + k] - m) * c;   // base-2 units
+      const float e = mine[k] >= 0 ? exp2f(z) : 0.0f;
+      ent[o + k] = {mine[k], e, z * kLn2, -1.0f};
+      s += e;
+    }
+    s = wsum(s);
+    const float ls = logf(s);
+    for (int k = lane; k < K; k += 32) {
+      ent[o + k].lp -= ls;
+      ent[o + k].p = ent[o + k].p == 0.0f ? 0.0f : ent[o + k].p / s;
+    }
+    __syncwarp();   // the other lanes' ids and p
+    for (int k = lane; k < K; k += 32) {
+      const int id = mine[k];
+      if (id < 0) continue;
+      float sum = ent[o + k].p;
+      for (int j = 0; j < K; ++j)
+        if (mine[j] == id && j != k) {
+          if (j < k) {
+            sum = -1.0f;
+            break;
+          }
+          sum += ent[o + j].p;
+        }
+      ent[o + k].own = sum;
+    }
+    __syncwarp();   // the ids are rewritten by the next row
+    if (lane == 0) flag[r] = any;
+    rows += any;
   }
-  if (lane == 0) sh[threadIdx.x >> 5] = c;
+  if (lane == 0) sh[threadIdx.x >> 5] = rows;
   __syncthreads();
   if (threadIdx.x == 0) {
-    c = 0;
-    for (int i = 0; i < 8; ++i) c += sh[i];
-    if (c) atomicAdd(count, c);
+    rows = 0;
+    for (int i = 0; i < 8; ++i) rows += sh[i];
+    if (rows) atomicAdd(count, rows);
   }
 }
 
-// The teacher's side of one row, by the block's first warp: p[k] (0 where there
-// is no entry) and whether there is any entry.  lp[k] = log p[k].
-__device__ __forceinline__ bool teacher_row(const void* ids, int idt, const float* teacher, int64_t r, int K, int64_t V,
-                                            float c, int64_t* id, float* p, float* lp) {
-  const int lane = threadIdx.x & 31;
-  float m = -INFINITY;
-  bool any = false;
-  for (int k = lane; k < K; k += 32) {
-    int64_t i = id_at(ids, idt, r * K + k);
-    const float te = teacher[r * K + k];
-    if (!entry_there(i, te, V)) i = -1;
-    id[k] = i;
-    p[k] = te;
-    if (i >= 0) {
-      m = fmaxf(m, te);
-      any = true;
-    }
-  }
-  m = wmax(m);
-  any = __any_sync(0xffffffffu, any);
-  float s = 0.0f;
-  for (int k = lane; k < K; k += 32) {
-    const float z = (p[k] - m) * c;   // base-2 units
-    const float e = id[k] >= 0 ? exp2f(z) : 0.0f;
-    lp[k] = z * kLn2;
-    p[k] = e;
-    s += e;
-  }
-  s = wsum(s);
-  const float ls = logf(s);
-  for (int k = lane; k < K; k += 32) {
-    lp[k] -= ls;
-    p[k] = id[k] >= 0 ? p[k] / s : 0.0f;
-  }
-  return any;
-}
+struct Distill {
+  const float* logits;
+  const Entry* ent;
+  const int *flag, *count;
+  int64_t rows, V;
+  int K;
+  float T;
+  float *part, *dl;   // part: [rows][parts], the row's kl in pieces
+  int parts;
+  int land;           // float4s of the landing buffer
+  int32_t* err;
+};
 
-__global__ void __launch_bounds__(kMaxThreads)
-k_distill_rows(const float* __restrict__ logits, int64_t V, const void* __restrict__ ids, int idt,
-               const float* __restrict__ teacher, int K, float T, const int* __restrict__ count,
-               float* __restrict__ kl, float* __restrict__ dl) {
-  __shared__ float red[64];
-  __shared__ float2 mine;
-  __shared__ int any_sh;
-  extern __shared__ int64_t dyn[];
-  int64_t* id = dyn;
-  float* p = reinterpret_cast<float*>(dyn + K);
-  float* lp = p + K;
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  const int64_t r = blockIdx.x / cs;
-  const float* row = logits + r * V;
-  const RowSlice sl = slice_of(row, V, rank, cs);
-  const float c = kLog2e / T;
-  float4 v[kNV];
-  int n = 0;
-#pragma unroll
-  for (int k = 0; k < kNV; ++k) {
-    const int64_t g = sl.g0 + (int64_t)k * blockDim.x + threadIdx.x;
-    if (g < sl.g1) {
-      v[k] = load_group(row, V, 4 * g - sl.shift);
-      n = k + 1;
-    }
-  }
-  if (threadIdx.x < 32) {
-    const bool any = teacher_row(ids, idt, teacher, r, K, V, c, id, p, lp);
-    if (threadIdx.x == 0) any_sh = any;
-  }
-  const RowStat st = row_stat(v, n, c, cl, red, &mine);   // its barriers also publish the teacher's side
-  const bool counted = any_sh != 0;
-  if (rank == 0 && threadIdx.x < 32) {
-    float s = 0.0f;
-    if (counted) {
-      const float lz = logf(st.sum);
-      for (int k = threadIdx.x; k < K; k += 32)
-        if (p[k] != 0.0f) s += p[k] * (lp[k] - ((row[id[k]] - st.max) * (c * kLn2) - lz));
-      s = wsum(s);
-    }
-    if (threadIdx.x == 0) kl[r] = s * (T * T);
-  }
-  if (!dl) return;
-  float* out = dl + r * V;
-  const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)sl.shift;
-  const float scale = T / (float)max(1, *count), inv = scale / st.sum;
+// q of the groups g + k * step in v into the row's gradient (`vec`: its groups
+// are aligned like the logits')
+__device__ __forceinline__ void distill_store(float* out, int V, const RowSlice& sl, const float4 (&v)[kNV], int n, int g,
+                                              int step, float f, bool vec) {
+  float4* base = reinterpret_cast<float4*>(out - sl.shift);
 #pragma unroll
   for (int k = 0; k < kNV; ++k)
     if (k < n) {
-      const int64_t e = 4 * (sl.g0 + (int64_t)k * blockDim.x + threadIdx.x) - sl.shift;
-      const float4 q = counted ? make_float4(v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv)
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
-      store_group(out, V, e, q, vec);
+      const int i = g + k * step;
+      const float4 q = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
+      if (vec && i >= sl.w0 && i < sl.w1) base[i] = q;
+      else store_edge(out, V, 4 * i - sl.shift, q);
     }
-  if (!counted) return;   // uniform over the cluster
-  // The teacher's entries, after the whole row is written.  An id listed more
-  // than once is handled by its first entry, which takes the others' p in order.
-  if (cs > 1) cl.sync();
-  else __syncthreads();
-  if (rank != 0) return;
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    if (id[k] < 0) continue;
-    bool first = true;
-    for (int j = 0; j < k && first; ++j) first = id[j] != id[k];
-    if (!first) continue;
-    float s = 0.0f;
-    for (int j = k; j < K; ++j)
-      if (id[j] == id[k]) s += p[j];
-    const float q = exp2f((row[id[k]] - st.max) * c) / st.sum;
-    out[id[k]] = scale * (q - s);
+}
+// The part of an entry with logit z in its row's kl.
+__device__ __forceinline__ float entry_kl(const Entry& e, float z, RowStat st, float log_sum, float inv_T) {
+  return e.p != 0.0f ? e.p * (e.lp - ((z - st.max) * inv_T - log_sum)) : 0.0f;
+}
+
+__global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill d) {
+  const int lane = threadIdx.x & 31, V = (int)d.V;
+  const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T;
+  for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < d.rows; r += (int64_t)gridDim.x * kWarps) {
+    const float* row = d.logits + r * d.V;
+    const RowSlice sl = slice_of(row, V, 0, 1);
+    const bool counted = d.flag[r];
+    float* out = d.dl + r * d.V;
+    if (!counted) {
+      if (lane == 0) d.part[r] = 0.0f;
+      if (d.dl)
+        for (int e = lane; e < V; e += 32) out[e] = 0.0f;
+      continue;
+    }
+    float4 v[kNV];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kNV; ++k) {
+      const int g = k * 32 + lane;
+      if (g < sl.g1) {
+        v[k] = g >= sl.w0 && g < sl.w1 ? sl.base[g] : load_edge(row, V, 4 * g - sl.shift);
+        n = k + 1;
+      }
+    }
+    const RowStat st = warp_stat(v, n, c);
+    const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)sl.shift;
+    if (d.dl) {
+      distill_store(out, V, sl, v, n, lane, 32, scale / st.sum, vec);
+      __syncwarp();   // the entries' columns are written again
+    }
+    const float ls = logf(st.sum), inv_T = 1.0f / d.T;
+    float kl = 0.0f;
+    for (int k = lane; k < d.K; k += 32) {
+      const Entry e = d.ent[r * d.K + k];
+      if (e.id < 0) continue;
+      const float z = row[e.id];
+      kl += entry_kl(e, z, st, ls, inv_T);
+      if (d.dl && e.own != -1.0f) out[e.id] = scale * (tc::exp2_hw((z - st.max) * c) / st.sum - e.own);
+    }
+    kl = wsum(kl);
+    if (lane == 0) d.part[r] = kl * (d.T * d.T);
   }
+}
+
+template <int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(const Distill d) {
+  extern __shared__ __align__(16) float4 land[];
+  __shared__ float2 table[2][kTable];
+  __shared__ uint64_t bar;
+  cg::cluster_group cl = cg::this_cluster();
+  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank(), V = (int)d.V;
+  const int64_t step = gridDim.x / cs;
+  Landing L;
+  L.init(land, &bar, d.err);
+  const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T;
+  int64_t r = blockIdx.x / cs;
+  RowSlice sl = slice_of(d.logits + r * d.V, V, rank, cs);
+  if (r < d.rows) L.issue(sl);
+  // Entry k of a row is thread k's (and k + blockDim.x, ...), in the block whose
+  // slice holds its column.  Its logit is read from the landing buffer and kept in
+  // ze; the first entry of the next row is fetched a row ahead.
+  float* ze = reinterpret_cast<float*>(land + d.land);
+  const int tid = (int)threadIdx.x, nt = (int)blockDim.x;
+  Entry first = {-1, 0.0f, 0.0f, -1.0f};
+  if (r < d.rows && tid < d.K) first = d.ent[r * d.K + tid];
+  const float inv_T = 1.0f / d.T;
+  int turn = 0;
+  for (; r < d.rows; r += step) {
+    const float* row = d.logits + r * d.V;
+    const RowSlice cur = sl;
+    const bool counted = d.flag[r];
+    L.wait();
+    if (cur.shift && L.holds(cur, 0)) land[0] = load_edge(row, V, -cur.shift);
+    if (L.holds(cur, cur.w1)) land[cur.w1 - cur.g0] = load_edge(row, V, 4 * cur.w1 - cur.shift);
+    float4 v[kNV];
+    const int n = L.take(v, cur);
+    // columns of this block's slice, and the buffer as floats from its first one
+    const int e0 = max(0, 4 * cur.g0 - cur.shift), e1 = min(V, 4 * cur.g1 - cur.shift);
+    const Entry mine = first;
+    if (counted)
+      for (int k = tid; k < d.K; k += nt) {
+        const int id = k == tid ? mine.id : d.ent[r * d.K + k].id;
+        // an element of a group that reaches past the row is another thread's to patch: from memory
+        if (id >= e0 && id < e1) {
+          const int q = id + cur.shift;
+          ze[k] = q >= 4 * cur.w0 && q < 4 * cur.w1 ? reinterpret_cast<const float*>(land)[q - 4 * cur.g0] : row[id];
+        }
+      }
+    __syncthreads();   // the buffer is free
+    if (r + step < d.rows) {
+      sl = slice_of(row + step * d.V, V, rank, cs);
+      L.issue(sl);
+      if (tid < d.K) first = d.ent[(r + step) * d.K + tid];
+    }
+    float* out = d.dl + r * d.V;
+    const int wp = (d.K + 31) / 32;   // warps of a block whose lanes have entries (at most all)
+    float* part = d.part + r * d.parts + rank * (d.parts / cs);
+    if (!counted) {
+      if (tid < d.parts / cs) part[tid] = 0.0f;
+      if (d.dl)
+        for (int e = e0 + tid; e < e1; e += nt) out[e] = 0.0f;
+      continue;   // uniform over the cluster
+    }
+    float f;
+    const RowStat st = join(warp_stat(v, n, c), c, cl, table[turn], &f);
+    turn ^= 1;
+    if (d.dl) {
+      const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)cur.shift;
+      distill_store(out, V, cur, v, n, cur.g0 + tid, nt, f * scale / st.sum, vec);
+      __syncthreads();   // the entries' columns are written again, by other threads of the block
+    }
+    if ((tid >> 5) < wp) {
+      const float ls = logf(st.sum);
+      float kl = 0.0f;
+      for (int k = tid; k < d.K; k += nt) {
+        const Entry e = k == tid ? mine : d.ent[r * d.K + k];
+        if (e.id < e0 || e.id >= e1) continue;
+        const float z = ze[k];
+        kl += entry_kl(e, z, st, ls, inv_T);
+        if (d.dl && e.own != -1.0f) out[e.id] = scale * (tc::exp2_hw((z - st.max) * c) / st.sum - e.own);
+      }
+      kl = wsum(kl);
+      if ((tid & 31) == 0) part[tid >> 5] = kl * (d.T * d.T);
+    }
+  }
+  if (cs > 1) cl.sync();   // no block leaves while another may write its table
 }
 
 // Blocks per row and threads per block for rows of `groups` 16-byte groups;
@@ -417,10 +647,13 @@ bool row_launch(int64_t groups, int* cs, int* threads) {
   return false;
 }
 
+// Blocks that stay: exactly as many clusters as the device holds at once (one
+// more would start when the others have walked all their rows).
+// `more`: dynamic shared memory behind the landing buffer.
 template <class K, class... A>
-void launch_rows(K kernel, int64_t rows, int cs, int threads, size_t smem, A... args) {
+void launch_rows(K kernel, int64_t rows, int64_t groups, int cs, int threads, size_t more, A... args) {
+  const size_t smem = (size_t)((groups + cs - 1) / cs) * 16 + more;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cs));
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream();
@@ -431,7 +664,26 @@ void launch_rows(K kernel, int64_t rows, int cs, int threads, size_t smem, A... 
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  // asked of the driver once per kernel and row length
+  static std::mutex mu;
+  static std::map<std::pair<int64_t, size_t>, int> resident;
+  static std::map<K, size_t> smem_set;
+  std::lock_guard<std::mutex> lk(mu);
+  if (size_t& most = smem_set[kernel]; smem > most) {
+    MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    most = smem;
+  }
+  int& res = resident[{groups, more}];
+  if (!res) {
+    cfg.gridDim = dim3((unsigned)(kNumSMs / cs * cs));
+    MALUS_CUDA(cudaOccupancyMaxActiveClusters(&res, kernel, &cfg));
+    if (res < 1) panic("softmax rows: no cluster of %d blocks can be resident", cs);
+  }
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, res) * cs));
   MALUS_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+unsigned warp_row_blocks(int64_t rows) {
+  return (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, kNumSMs * 4);
 }
 
 }  // namespace
@@ -446,9 +698,11 @@ void xent_rows(float* logits, int64_t ld, int64_t n, int64_t V, const void* targ
                float* nll) {
   if (n == 0) return;
   int cs, threads;
-  if (!row_launch(ld / 4, &cs, &threads)) panic("xent_rows: rows of %lld logits", (long long)V);
   const int pid = prof_begin_named("k_xent_rows", 8.0 * (double)n * (double)ld);
-  launch_rows(k_xent_rows, n, cs, threads, 0, logits, ld, V, targets, tgt_dtype, row0, nll);
+  if (ld <= kShort)
+    k_xent_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(logits, (int)ld, n, (int)V, targets, tgt_dtype, row0, nll);
+  else if (!row_launch(ld / 4, &cs, &threads)) panic("softmax rows of %lld logits", (long long)V);
+  else launch_rows(threads > kThreads ? k_xent_rows<kMaxThreads> : k_xent_rows<kThreads>, n, ld / 4, cs, threads, 0, logits, (int)ld, n, (int)V, targets, tgt_dtype, row0, nll, device_error_word());
   count_launch();
   after_launch("k_xent_rows");
   prof_end(pid);
@@ -462,8 +716,8 @@ void xent_join(const float2* part, int parts, const float* at, const void* targe
   after_launch("k_xent_join");
 }
 
-void loss_mean(const float* v, int64_t n, const int* count, float* loss) {
-  k_loss_mean<<<1, 1024, 0, stream()>>>(v, n, count, loss);
+void loss_mean(float* v, int64_t n, const int* count, float* loss) {
+  k_loss_mean<<<1, 1024, 0, stream()>>>(v, nullptr, 0, n, count, loss);
   count_launch();
   after_launch("k_loss_mean");
 }
@@ -490,9 +744,7 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   const int64_t n = (int64_t)s.d[0], V = (int64_t)s.d[1], K = (int64_t)si.d[1];
   if (V == 0) panic("distill over an empty vocabulary");
   if (K < 1 || K > kMaxEntries) panic("distill takes 1 to %d teacher entries per row, got %lld", kMaxEntries, (long long)K);
-  int cs, threads;
-  // a row may start up to 3 elements past an aligned address
-  if (V > kMaxRowLogits - 4 || !row_launch((V + 3 + 3) / 4, &cs, &threads))
+  if (V > kMaxRowLogits - 4)
     panic("distill rows are limited to %lld logits, got %lld", (long long)kMaxRowLogits - 4, (long long)V);
   if (n > (int64_t)1 << 27) panic("distill is limited to 2^27 rows, got %lld", (long long)n);
   const float* x = fptr(logits);
@@ -500,20 +752,37 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   const float* te = fptr(teacher);
   const int64_t loss = alloc_f32({1}), hk = alloc_f32({s.d[0]});
   const int64_t hd = dlogits ? alloc_shape(s) : 0;
-  int* count = static_cast<int*>(scratch_alloc(4));
+  // a row may start 3 past an aligned address
+  const int64_t groups = (V + 3 + 3) / 4;
+  int cs = 1, threads = 0, parts = 1;
+  if (V > kShort) {
+    if (!row_launch(groups, &cs, &threads)) panic("softmax rows of %lld logits", (long long)V);
+    parts = cs * std::min((int)(K + 31) / 32, threads / 32);
+  }
+  char* ws = static_cast<char*>(scratch_alloc(16 + (size_t)(n * K) * sizeof(Entry) + (size_t)n * 4 * (1 + parts)));
+  int* count = reinterpret_cast<int*>(ws);
+  Entry* ent = reinterpret_cast<Entry*>(ws + 16);
+  int* flag = reinterpret_cast<int*>(ent + n * K);
+  float* part = reinterpret_cast<float*>(flag + n);
   MALUS_CUDA(cudaMemsetAsync(count, 0, 4, stream()));
   if (n) {
-    k_distill_count<<<grid_for((size_t)n * 32, 256), 256, 0, stream()>>>(idp, idt, te, n, (int)K, V, count,
-                                                                        device_error_word());
+    const int land = (int)((groups + cs - 1) / cs);
+    const Distill d{x, ent, flag, count, n, V, (int)K, temperature, part, hd ? fptr(hd) : nullptr, parts, land,
+                    device_error_word()};
+    k_teacher<<<grid_for((size_t)n * 32, 256), 256, (size_t)K * 32, stream()>>>(
+        idp, idt, te, n, (int)K, V, kLog2e / temperature, ent, flag, count, device_error_word());
     const int pid = prof_begin_named("k_distill_rows", (hd ? 8.0 : 4.0) * (double)n * (double)V);
-    launch_rows(k_distill_rows, n, cs, threads, (size_t)K * 16, x, V, idp, idt, te, (int)K, temperature,
-                (const int*)count, fptr(hk), hd ? fptr(hd) : (float*)nullptr);
+    if (V <= kShort) k_distill_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(d);
+    else launch_rows(threads > kThreads ? k_distill_rows<kMaxThreads> : k_distill_rows<kThreads>, n, groups, cs, threads,
+                     (size_t)K * 4, d);
     count_launch(2);
     after_launch("k_distill_rows");
     prof_end(pid);
   }
-  loss_mean(fptr(hk), n, count, fptr(loss));
-  scratch_free(count);
+  k_loss_mean<<<1, 1024, 0, stream()>>>(fptr(hk), part, parts, n, count, fptr(loss));
+  count_launch();
+  after_launch("k_loss_mean");
+  scratch_free(ws);
   if (kl) *kl = hk;
   else tensor_release(hk);
   if (dlogits) *dlogits = hd;

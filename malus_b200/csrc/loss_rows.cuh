@@ -23,7 +23,7 @@ void xent_join(const float2* part, int parts, const float* at, const void* targe
                float* nll);
 
 // loss[0] = sum of v[0 .. n) / max(1, count[0])
-void loss_mean(const float* v, int64_t n, const int* count, float* loss);
+void loss_mean(float* v, int64_t n, const int* count, float* loss);
 
 constexpr int64_t kMaxRowLogits = 262144;   // longest row (pitch) xent_rows takes
 
