@@ -59,15 +59,16 @@ struct RowSlice {
   int g0, g1;           // this block's groups
   int w0, w1;
 };
-__device__ __forceinline__ RowSlice slice_of(const float* row, int V, int rank, int cs) {
+// (the cluster has 2^lc blocks)
+__device__ __forceinline__ RowSlice slice_of(const float* row, int V, int rank, int lc) {
   RowSlice s;
   s.shift = (int)(((uintptr_t)row >> 2) & 3);
   s.base = reinterpret_cast<const float4*>(row - s.shift);
-  const int groups = (V + s.shift + 3) / 4, per = (groups + cs - 1) / cs;
+  const int groups = (V + s.shift + 3) >> 2, per = (groups + (1 << lc) - 1) >> lc;
   s.g0 = min(rank * per, groups);
   s.g1 = min(s.g0 + per, groups);
   s.w0 = s.shift ? 1 : 0;
-  s.w1 = (V + s.shift) / 4;
+  s.w1 = (V + s.shift) >> 2;
   return s;
 }
 __device__ __forceinline__ float4 load_edge(const float* __restrict__ row, int V, int e) {
@@ -82,32 +83,30 @@ __device__ __forceinline__ void store_edge(float* __restrict__ row, int V, int e
   if (e + 3 >= 0 && e + 3 < V) row[e + 3] = q.w;
 }
 
-// Maximum and sum of exponentials of a row whose groups the threads hold in v
-// (n of them in this thread): v becomes exp((v - max) * c) after row_scale, and
-// the sum is over the whole row.  Elements of -inf give 0; a row of -inf only, or
-// with a +inf or NaN, gives NaN probabilities as the formula does.
+// Maximum and sum of exponentials of a row whose groups the threads hold in v,
+// -inf where a thread has none: v becomes exp((v - max) * c) after the join below,
+// and the sum is over the whole row.  Elements of -inf give 0; a row of -inf only,
+// or with a +inf or NaN, gives NaN probabilities as the formula does.
 struct RowStat { float max, sum; };
 
 // The warp's maximum; v becomes exp against it and the sum is the warp's.  The
 // exponential is the hardware's base-2 one (relative error 2^-22; results
 // below 2^-126 are 0).
-__device__ __forceinline__ RowStat warp_stat(float4 (&v)[kNV], int n, float c) {
+__device__ __forceinline__ RowStat warp_stat(float4 (&v)[kNV], float c) {
   float m = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kNV; ++k)
-    if (k < n) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+  for (int k = 0; k < kNV; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
   m = wmax(m);
   const float m0 = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kNV; ++k)
-    if (k < n) {
-      v[k].x = tc::exp2_hw((v[k].x - m0) * c);
-      v[k].y = tc::exp2_hw((v[k].y - m0) * c);
-      v[k].z = tc::exp2_hw((v[k].z - m0) * c);
-      v[k].w = tc::exp2_hw((v[k].w - m0) * c);
-      s += (v[k].x + v[k].y) + (v[k].z + v[k].w);
-    }
+  for (int k = 0; k < kNV; ++k) {
+    v[k].x = tc::exp2_hw((v[k].x - m0) * c);
+    v[k].y = tc::exp2_hw((v[k].y - m0) * c);
+    v[k].z = tc::exp2_hw((v[k].z - m0) * c);
+    v[k].w = tc::exp2_hw((v[k].w - m0) * c);
+    s += (v[k].x + v[k].y) + (v[k].z + v[k].w);
+  }
   return {m, wsum(s)};
 }
 // a part of -inf only has the sum 0 (or NaN) whatever its factor
@@ -115,34 +114,77 @@ __device__ __forceinline__ float join_factor(float m, float M, float c) {
   return m == -INFINITY ? 1.0f : tc::exp2_hw((m - M) * c);
 }
 
-// Joins the warps of a cluster of blocks (or of one block): every warp writes its
-// pair into each block's table, one barrier, and every warp reduces the table.
-// `f` is what brings this warp's exponentials to the row's maximum.  Two tables
-// alternate: with one cluster barrier per row nobody overwrites one that another
-// warp may still read.  Every block has its slice in registers when this returns.
-__device__ __forceinline__ RowStat join(RowStat w, float c, cg::cluster_group& cl, float2* table, float* f) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int cs = (int)cl.num_blocks(), total = cs * warps;
-  if (cs == 1) {
-    if (lane == 0) table[warp] = make_float2(w.max, w.sum);
-    __syncthreads();
-  } else {
-    if (lane < cs) *cl.map_shared_rank(table + cl.block_rank() * warps + warp, lane) = make_float2(w.max, w.sum);
-    cl.sync();
-  }
-  float M = -INFINITY;
-  for (int i = lane; i < total; i += 32) M = fmaxf(M, table[i].x);
-  M = wmax(M);
-  float S = 0.0f;
-  for (int i = lane; i < total; i += 32) S += table[i].y * join_factor(table[i].x, M, c);
-  *f = join_factor(w.max, M, c);
-  return {M, wsum(S)};
+// A wait of at most the bound; false (and an error word of `code`) when it runs out.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int32_t* err, int code) {
+  if (tc::mbar_try(bar, parity)) return true;
+  const uint64_t t0 = tc::gtimer();
+  while (!tc::mbar_try(bar, parity))
+    if (tc::gtimer() - t0 > tc::kWaitNs) {
+      atomicExch(err, code);
+      return false;
+    }
+  return true;
 }
+
 constexpr int kTable = kMaxCluster * kMaxThreads / 32;
+// Joins the warps of a cluster of blocks (or of one block).  Every warp sends its
+// pair into each block's table by an asynchronous store that counts on that
+// block's barrier, and every warp waits for its own block's barrier and reduces
+// the table.  (A cluster barrier in its place also waits until the gradient
+// stores of the row before are acknowledged.)  Two tables alternate: a warp sends
+// into one again only after it has every block's pairs of the row between, which
+// they send when they are done with this one.
+struct Join {
+  float2* table;     // [2][kTable]
+  uint32_t bar[2];
+  uint32_t uses;
+  bool dead;
+  int32_t* err;
+
+  __device__ __forceinline__ void init(float2* t, uint64_t* bars, int32_t* e, cg::cluster_group& cl) {
+    table = t;
+    uses = 0;
+    dead = false;
+    err = e;
+    for (int i = 0; i < 2; ++i) {
+      bar[i] = tc::smem_u32(bars + i);
+      if (threadIdx.x == 0) tc::mbar_init(bar[i], 1);
+    }
+    if (threadIdx.x == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    cl.sync();   // every block's barriers exist before another counts on them
+  }
+  // `f` is what brings this warp's exponentials to the row's maximum.
+  __device__ __forceinline__ RowStat operator()(RowStat w, float c, cg::cluster_group& cl, float* f) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int cs = (int)cl.num_blocks(), total = cs * warps, turn = uses & 1;
+    float2* t = table + turn * kTable;
+    if (cs == 1) {
+      if (lane == 0) t[warp] = make_float2(w.max, w.sum);
+      __syncthreads();
+    } else {
+      if (threadIdx.x == 0) tc::mbar_expect_tx(bar[turn], (uint32_t)total * 8);
+      if (lane < cs) {
+        const uint64_t v = ((uint64_t)__float_as_uint(w.sum) << 32) | __float_as_uint(w.max);
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];"
+                     ::"r"(tc::cluster_addr(tc::smem_u32(t + cl.block_rank() * warps + warp), lane)), "l"(v),
+                       "r"(tc::cluster_addr(bar[turn], lane))
+                     : "memory");
+      }
+      if (!dead) dead = !wait_for(bar[turn], (uses >> 1) & 1, err, 52);
+    }
+    ++uses;
+    float M = -INFINITY;
+    for (int i = lane; i < total; i += 32) M = fmaxf(M, t[i].x);
+    M = wmax(M);
+    float S = 0.0f;
+    for (int i = lane; i < total; i += 32) S += t[i].y * join_factor(t[i].x, M, c);
+    *f = join_factor(w.max, M, c);
+    return {M, wsum(S)};
+  }
+};
 
 // The landing buffer: the slice of the next row, brought by a bulk copy of its
-// whole 16-byte groups (the groups that reach past the row are read from memory
-// by the thread that holds them).  A copy that does not arrive within the wait's
+// whole 16-byte groups.  A copy that does not arrive within the wait's
 // bound is reported in the error word; no further copy is then issued or waited for.
 struct Landing {
   float4* buf;
@@ -175,29 +217,22 @@ struct Landing {
   }
   __device__ __forceinline__ void wait() {
     if (dead) return;
-    if (!tc::mbar_try(bar, parity)) {
-      const uint64_t t0 = tc::gtimer();
-      while (!tc::mbar_try(bar, parity))
-        if (tc::gtimer() - t0 > tc::kWaitNs) {
-          dead = true;
-          atomicExch(err, 51);
-          break;
-        }
-    }
+    dead = !wait_for(bar, parity, err, 51);
     parity ^= 1;
   }
-  // whether this thread holds group g of the slice
-  __device__ __forceinline__ bool holds(const RowSlice& s, int g) const {
-    return g >= s.g0 && g < s.g1 && (g - s.g0) % (int)blockDim.x == (int)threadIdx.x;
-  }
-  // this thread's groups of the landed slice into v; returns how many
-  __device__ __forceinline__ int take(float4 (&v)[kNV], const RowSlice& s) const {
+  // this thread's groups t + k * blockDim.x of the landed slice into v, -inf past
+  // its end; a group that reaches past the row (first, last) comes from memory
+  __device__ __forceinline__ void take(float4 (&v)[kNV], const RowSlice& s, const float* row, int V) const {
     const int len = s.g1 - s.g0, nt = (int)blockDim.x, t = (int)threadIdx.x;
-    const int n = len > t ? (len - t + nt - 1) / nt : 0;
+    const int last = s.w1 < s.g1 ? s.w1 - s.g0 : -1;
+    const bool head = s.shift && s.g0 == 0;
 #pragma unroll
-    for (int k = 0; k < kNV; ++k)
-      if (k < n) v[k] = buf[t + k * nt];
-    return n;
+    for (int k = 0; k < kNV; ++k) {
+      const int i = t + k * nt;
+      v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (i < len) v[k] = buf[i];
+      if (i == last || (head && i == 0)) v[k] = load_edge(row, V, 4 * (s.g0 + i) - s.shift);
+    }
   }
 };
 
@@ -219,12 +254,12 @@ __device__ __forceinline__ void store_planes(float* row, int ld, int e, float4 q
 }
 
 // the gradient of a row's groups that this thread holds in v (exponentials):
-// group g + k * step
-__device__ __forceinline__ void xent_store(float* row, int ld, const float4 (&v)[kNV], int n, int g, int step,
-                                           float f, int t) {
+// groups g + k * step below g1
+__device__ __forceinline__ void xent_store(float* row, int ld, const float4 (&v)[kNV], int g, int g1, int step, float f,
+                                           int t) {
 #pragma unroll
   for (int k = 0; k < kNV; ++k)
-    if (k < n) {
+    if (g + k * step < g1) {
       const int e = 4 * (g + k * step);
       float4 q = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
       const unsigned o = (unsigned)(t - e);
@@ -257,18 +292,15 @@ k_xent_rows_warp(float* __restrict__ logits, int ld, int64_t rows, int V, const 
     }
     const float zt = row[t];
     float4 v[kNV];
-    int n = 0;
 #pragma unroll
     for (int k = 0; k < kNV; ++k) {
       const int g = k * 32 + lane;
-      if (g < ld / 4) {
-        v[k] = cut_group(reinterpret_cast<const float4*>(row)[g], 4 * g, V);
-        n = k + 1;
-      }
+      v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (4 * g < V) v[k] = cut_group(reinterpret_cast<const float4*>(row)[g], 4 * g, V);
     }
-    const RowStat st = warp_stat(v, n, kLog2e);   // the whole row is in registers after it
+    const RowStat st = warp_stat(v, kLog2e);   // the whole row is in registers after it
     if (lane == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
-    xent_store(row, ld, v, n, lane, 32, 1.0f / st.sum, (int)t);
+    xent_store(row, ld, v, lane, ld / 4, 32, 1.0f / st.sum, (int)t);
   }
 }
 
@@ -277,17 +309,18 @@ __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2)
 k_xent_rows(float* __restrict__ logits, int ld, int64_t rows, int V, const void* __restrict__ tgt, int tdt,
             int64_t row0, float* __restrict__ nll, int32_t* __restrict__ err) {
   extern __shared__ __align__(16) float4 land[];
-  __shared__ float2 table[2][kTable];
-  __shared__ uint64_t bar;
+  __shared__ float2 table[2 * kTable];
+  __shared__ uint64_t bar, jbar[2];
   cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  const int64_t step = gridDim.x / cs;
+  const int cs = (int)cl.num_blocks(), lc = 31 - __clz(cs), rank = (int)cl.block_rank();
+  const int64_t step = gridDim.x >> lc;
   Landing L;
   L.init(land, &bar, err);
-  int64_t r = blockIdx.x / cs;
-  RowSlice sl = slice_of(logits + r * ld, ld, rank, cs);   // the pitch is whole groups: the same in every row
+  Join join;
+  join.init(table, jbar, err, cl);
+  int64_t r = blockIdx.x >> lc;
+  RowSlice sl = slice_of(logits + r * ld, ld, rank, lc);   // the pitch is whole groups: the same in every row
   if (r < rows) L.issue(sl);
-  int turn = 0;
   for (; r < rows; r += step) {
     float* row = logits + r * ld;
     const int64_t t = id_at(tgt, tdt, row0 + r);
@@ -295,28 +328,33 @@ k_xent_rows(float* __restrict__ logits, int ld, int64_t rows, int V, const void*
     float zt = 0.0f;
     if (counted && rank == 0 && threadIdx.x == 0) zt = row[t];
     L.wait();
-    for (int g = V / 4; g < sl.g1; ++g)   // what lies behind the row is no logit (at most 16 groups)
-      if (L.holds(sl, g)) land[g - sl.g0] = cut_group(land[g - sl.g0], 4 * g, V);
+    const int g = sl.g0 + (int)threadIdx.x;
     float4 v[kNV];
-    const int n = L.take(v, sl);
+    L.take(v, sl, row, ld);
+    if (4 * sl.g1 > V) {   // what lies behind the row is no logit
+#pragma unroll
+      for (int k = 0; k < kNV; ++k) {
+        const int e = 4 * (g + k * (int)blockDim.x);
+        if (e + 4 > V) v[k] = cut_group(v[k], e, V);
+      }
+    }
     __syncthreads();   // the buffer is free
     sl.base += step * (ld / 4);
     if (r + step < rows) L.issue(sl);
-    const int g = sl.g0 + (int)threadIdx.x;
     if (counted) {
       float f;
-      const RowStat st = join(warp_stat(v, n, kLog2e), kLog2e, cl, table[turn], &f);
-      turn ^= 1;
+      const RowStat st = join(warp_stat(v, kLog2e), kLog2e, cl, &f);
       if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = logf(st.sum) - (zt - st.max);
-      xent_store(row, ld, v, n, g, blockDim.x, f / st.sum, (int)t);
+      xent_store(row, ld, v, g, sl.g1, blockDim.x, f / st.sum, (int)t);
     } else {
       if (rank == 0 && threadIdx.x == 0) nll[row0 + r] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kNV; ++k)
-        if (k < n) store_planes(row, ld, 4 * (g + k * (int)blockDim.x), make_float4(0.f, 0.f, 0.f, 0.f));
+        if (g + k * (int)blockDim.x < sl.g1)
+          store_planes(row, ld, 4 * (g + k * (int)blockDim.x), make_float4(0.f, 0.f, 0.f, 0.f));
     }
   }
-  if (cs > 1) cl.sync();   // no block leaves while another may write its table
+  if (cs > 1) cl.sync();   // no block leaves while another may still send to it
 }
 
 __global__ void __launch_bounds__(1024) k_xent_count(const void* __restrict__ tgt, int tdt, int64_t n, int64_t V,
@@ -477,23 +515,26 @@ struct Distill {
   const float* logits;
   const Entry* ent;
   const int *flag, *count;
-  int64_t rows, V;
+  int64_t rows, V_;
   int K;
   float T;
   float *part, *dl;   // part: [rows][parts], the row's kl in pieces
   int parts;
   int land;           // float4s of the landing buffer
   int32_t* err;
+  __device__ __forceinline__ const float* row(int64_t r) const { return logits + r * V_; }
+  __device__ __forceinline__ int width() const { return (int)V_; }
+  __device__ __forceinline__ int V() const { return (int)V_; }
 };
 
 // q of the groups g + k * step in v into the row's gradient (`vec`: its groups
 // are aligned like the logits')
-__device__ __forceinline__ void distill_store(float* out, int V, const RowSlice& sl, const float4 (&v)[kNV], int n, int g,
+__device__ __forceinline__ void distill_store(float* out, int V, const RowSlice& sl, const float4 (&v)[kNV], int g,
                                               int step, float f, bool vec) {
   float4* base = reinterpret_cast<float4*>(out - sl.shift);
 #pragma unroll
   for (int k = 0; k < kNV; ++k)
-    if (k < n) {
+    if (g + k * step < sl.g1) {
       const int i = g + k * step;
       const float4 q = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
       if (vec && i >= sl.w0 && i < sl.w1) base[i] = q;
@@ -506,13 +547,13 @@ __device__ __forceinline__ float entry_kl(const Entry& e, float z, RowStat st, f
 }
 
 __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill d) {
-  const int lane = threadIdx.x & 31, V = (int)d.V;
+  const int lane = threadIdx.x & 31, V = (int)d.V_;
   const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T;
   for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < d.rows; r += (int64_t)gridDim.x * kWarps) {
-    const float* row = d.logits + r * d.V;
-    const RowSlice sl = slice_of(row, V, 0, 1);
+    const float* row = d.logits + r * d.V_;
+    const RowSlice sl = slice_of(row, V, 0, 0);
     const bool counted = d.flag[r];
-    float* out = d.dl + r * d.V;
+    float* out = d.dl + r * d.V_;
     if (!counted) {
       if (lane == 0) d.part[r] = 0.0f;
       if (d.dl)
@@ -520,19 +561,17 @@ __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill
       continue;
     }
     float4 v[kNV];
-    int n = 0;
 #pragma unroll
     for (int k = 0; k < kNV; ++k) {
       const int g = k * 32 + lane;
-      if (g < sl.g1) {
-        v[k] = g >= sl.w0 && g < sl.w1 ? sl.base[g] : load_edge(row, V, 4 * g - sl.shift);
-        n = k + 1;
-      }
+      v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (g >= sl.w0 && g < sl.w1) v[k] = sl.base[g];
+      else if (g < sl.g1) v[k] = load_edge(row, V, 4 * g - sl.shift);
     }
-    const RowStat st = warp_stat(v, n, c);
+    const RowStat st = warp_stat(v, c);
     const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)sl.shift;
     if (d.dl) {
-      distill_store(out, V, sl, v, n, lane, 32, scale / st.sum, vec);
+      distill_store(out, V, sl, v, lane, 32, scale / st.sum, vec);
       __syncwarp();   // the entries' columns are written again
     }
     const float ls = logf(st.sum), inv_T = 1.0f / d.T;
@@ -552,16 +591,18 @@ __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill
 template <int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(const Distill d) {
   extern __shared__ __align__(16) float4 land[];
-  __shared__ float2 table[2][kTable];
-  __shared__ uint64_t bar;
+  __shared__ float2 table[2 * kTable];
+  __shared__ uint64_t bar, jbar[2];
   cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank(), V = (int)d.V;
-  const int64_t step = gridDim.x / cs;
+  const int cs = (int)cl.num_blocks(), lc = 31 - __clz(cs), rank = (int)cl.block_rank(), V = (int)d.V_;
+  const int64_t step = gridDim.x >> lc;
   Landing L;
   L.init(land, &bar, d.err);
+  Join join;
+  join.init(table, jbar, d.err, cl);
   const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T;
-  int64_t r = blockIdx.x / cs;
-  RowSlice sl = slice_of(d.logits + r * d.V, V, rank, cs);
+  int64_t r = blockIdx.x >> lc;
+  RowSlice sl = slice_of(d.logits + r * d.V_, V, rank, lc);
   if (r < d.rows) L.issue(sl);
   // Entry k of a row is thread k's (and k + blockDim.x, ...), in the block whose
   // slice holds its column.  Its logit is read from the landing buffer and kept in
@@ -571,23 +612,20 @@ __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(
   Entry first = {-1, 0.0f, 0.0f, -1.0f};
   if (r < d.rows && tid < d.K) first = d.ent[r * d.K + tid];
   const float inv_T = 1.0f / d.T;
-  int turn = 0;
   for (; r < d.rows; r += step) {
-    const float* row = d.logits + r * d.V;
+    const float* row = d.logits + r * d.V_;
     const RowSlice cur = sl;
     const bool counted = d.flag[r];
     L.wait();
-    if (cur.shift && L.holds(cur, 0)) land[0] = load_edge(row, V, -cur.shift);
-    if (L.holds(cur, cur.w1)) land[cur.w1 - cur.g0] = load_edge(row, V, 4 * cur.w1 - cur.shift);
     float4 v[kNV];
-    const int n = L.take(v, cur);
+    L.take(v, cur, row, V);
     // columns of this block's slice, and the buffer as floats from its first one
     const int e0 = max(0, 4 * cur.g0 - cur.shift), e1 = min(V, 4 * cur.g1 - cur.shift);
     const Entry mine = first;
     if (counted)
       for (int k = tid; k < d.K; k += nt) {
         const int id = k == tid ? mine.id : d.ent[r * d.K + k].id;
-        // an element of a group that reaches past the row is another thread's to patch: from memory
+        // a group that reaches past the row did not land
         if (id >= e0 && id < e1) {
           const int q = id + cur.shift;
           ze[k] = q >= 4 * cur.w0 && q < 4 * cur.w1 ? reinterpret_cast<const float*>(land)[q - 4 * cur.g0] : row[id];
@@ -595,11 +633,11 @@ __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(
       }
     __syncthreads();   // the buffer is free
     if (r + step < d.rows) {
-      sl = slice_of(row + step * d.V, V, rank, cs);
+      sl = slice_of(row + step * d.V_, V, rank, lc);
       L.issue(sl);
       if (tid < d.K) first = d.ent[(r + step) * d.K + tid];
     }
-    float* out = d.dl + r * d.V;
+    float* out = d.dl + r * d.V_;
     const int wp = (d.K + 31) / 32;   // warps of a block whose lanes have entries (at most all)
     float* part = d.part + r * d.parts + rank * (d.parts / cs);
     if (!counted) {
@@ -609,11 +647,10 @@ __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(
       continue;   // uniform over the cluster
     }
     float f;
-    const RowStat st = join(warp_stat(v, n, c), c, cl, table[turn], &f);
-    turn ^= 1;
+    const RowStat st = join(warp_stat(v, c), c, cl, &f);
     if (d.dl) {
       const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)cur.shift;
-      distill_store(out, V, cur, v, n, cur.g0 + tid, nt, f * scale / st.sum, vec);
+      distill_store(out, V, cur, v, cur.g0 + tid, nt, f * scale / st.sum, vec);
       __syncthreads();   // the entries' columns are written again, by other threads of the block
     }
     if ((tid >> 5) < wp) {
@@ -630,7 +667,274 @@ __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : 2) k_distill_rows(
       if ((tid & 31) == 0) part[tid >> 5] = kl * (d.T * d.T);
     }
   }
-  if (cs > 1) cl.sync();   // no block leaves while another may write its table
+  if (cs > 1) cl.sync();   // no block leaves while another may still send to it
+}
+
+// ---- rows that fit a block's shared memory ----
+// A row of up to kRingGroups 16-byte groups lies whole in shared memory, in chunks
+// of two groups per thread.  One warp feeds it: as soon as every other warp is done
+// with a chunk, the same chunk of the block's next row is on its way.  The other
+// warps pass over the row twice: maximum and sum of exponentials as the chunks
+// arrive, then the gradient.  Reads of the next row overlap the second pass and its
+// stores, and nothing but one block barrier per row joins the warps.
+constexpr int kRingWarps = 24, kRingChunks = 16;
+constexpr int kRingGroups = 225 * 64;   // 225 KB
+
+struct Ring {
+  float4* row;                // [groups]
+  uint32_t full, empty;       // kRingChunks barriers each
+  int chunk, chunks, groups;  // groups: the row's, for any alignment
+  uint32_t parity;            // of the row being read
+  bool dead;
+  int32_t* err;
+
+  __device__ __forceinline__ uint32_t full_of(int j) const { return full + 8 * j; }
+  __device__ __forceinline__ uint32_t empty_of(int j) const { return empty + 8 * j; }
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t par, int code) {
+    if (!dead) dead = !wait_for(bar, par, err, code);
+  }
+  __device__ __forceinline__ void release(int j) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(empty_of(j));
+  }
+};
+
+// The feeding warp: rows first, first + step, ... below rows.
+template <class Op>
+__device__ __forceinline__ void ring_feed(Ring& R, const Op& op, int64_t first, int64_t step) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = first, it = 0; r < op.rows && !R.dead; r += step, ++it) {
+    const RowSlice s = slice_of(op.row(r), op.width(), 0, 0);
+    for (int j = 0; j < R.chunks; ++j) {
+      if (it) R.wait(R.empty_of(j), (uint32_t)(it - 1) & 1, 53);
+      if (R.dead) break;
+      const int lo = j * R.chunk, hi = min(lo + R.chunk, R.groups);
+      // groups that are not four logits of the row: written by element, -inf past its end
+      const int w0 = s.w0, w1 = (op.V() + s.shift) >> 2;
+      if (lane == 0 && lo == 0 && w0) R.row[0] = load_edge(op.row(r), op.V(), -s.shift);
+      for (int g = max(lo, w1) + lane; g < hi; g += 32) R.row[g] = load_edge(op.row(r), op.V(), 4 * g - s.shift);
+      __syncwarp();
+      if (lane == 0) {
+        const int i0 = max(lo, w0), i1 = min(hi, w1);
+        const uint32_t bytes = i1 > i0 ? (uint32_t)(i1 - i0) * 16 : 0;
+        tc::mbar_expect_tx(R.full_of(j), bytes);
+        if (bytes)
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(tc::smem_u32(R.row + i0)), "l"(s.base + i0), "r"(bytes), "r"(R.full_of(j))
+                       : "memory");
+      }
+    }
+  }
+}
+
+// First pass over the landed row: its maximum and sum, in every thread.  With
+// `once` the chunks are given back as they are read.
+__device__ __forceinline__ RowStat ring_stat(Ring& R, float c, float2* table, bool once) {
+  const int tid = (int)threadIdx.x, nt = R.chunk / 2, lane = tid & 31, warps = nt >> 5;
+  const float ninf = -INFINITY;
+  float m = ninf, s = 0.0f;
+  for (int j = 0; j < R.chunks; ++j) {
+    R.wait(R.full_of(j), R.parity, 54);
+    const int g = j * R.chunk + tid;
+    float4 a = make_float4(ninf, ninf, ninf, ninf), b = a;
+    if (g < R.groups) a = R.row[g];
+    if (g + nt < R.groups) b = R.row[g + nt];
+    if (once) R.release(j);
+    const float mx = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
+    const float mn = fmaxf(m, mx), m0 = mn == ninf ? 0.0f : mn;
+    s *= tc::exp2_hw((m - m0) * c);
+    m = mn;
+    s += ((tc::exp2_hw((a.x - m0) * c) + tc::exp2_hw((a.y - m0) * c)) +
+          (tc::exp2_hw((a.z - m0) * c) + tc::exp2_hw((a.w - m0) * c))) +
+         ((tc::exp2_hw((b.x - m0) * c) + tc::exp2_hw((b.y - m0) * c)) +
+          (tc::exp2_hw((b.z - m0) * c) + tc::exp2_hw((b.w - m0) * c)));
+  }
+  float2* t = table + R.parity * kRingWarps;   // two alternate: the barrier between keeps them apart
+  float M = wmax(m);
+  s = wsum(s * join_factor(m, M, c));
+  if (lane == 0) t[tid >> 5] = make_float2(M, s);
+  asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory");
+  const float2 o = lane < warps ? t[lane] : make_float2(ninf, 0.0f);
+  M = wmax(o.x);
+  return {M, wsum(o.y * join_factor(o.x, M, c))};
+}
+
+// Second pass: f(group, its four exponentials exp((x - max) * c)), chunk by chunk.
+template <class F>
+__device__ __forceinline__ void ring_map(Ring& R, RowStat st, float c, F&& f) {
+  const int tid = (int)threadIdx.x, nt = R.chunk / 2;
+  const float m0 = st.max == -INFINITY ? 0.0f : st.max;
+  for (int j = 0; j < R.chunks; ++j) {
+    const int g = j * R.chunk + tid;
+    float4 q[2];
+    if (g < R.groups) q[0] = R.row[g];
+    if (g + nt < R.groups) q[1] = R.row[g + nt];
+    R.release(j);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (g + i * nt < R.groups)
+        f(g + i * nt, make_float4(tc::exp2_hw((q[i].x - m0) * c), tc::exp2_hw((q[i].y - m0) * c),
+                                  tc::exp2_hw((q[i].z - m0) * c), tc::exp2_hw((q[i].w - m0) * c)));
+  }
+}
+
+struct XentRows {
+  float* logits;
+  int ld, V_;
+  int64_t rows;
+  const void* tgt;
+  int tdt;
+  int64_t row0;
+  float* nll;
+  int32_t* err;
+  __device__ __forceinline__ float* row(int64_t r) const { return logits + r * ld; }
+  __device__ __forceinline__ int width() const { return ld; }   // groups cover the pitch
+  __device__ __forceinline__ int V() const { return V_; }       // logits among them
+};
+
+__device__ __forceinline__ void ring_rows(Ring& R, const XentRows& d, float2* table, int64_t first, int64_t step) {
+  const int tid = (int)threadIdx.x, nt = R.chunk / 2;
+  int64_t next = first < d.rows ? id_at(d.tgt, d.tdt, d.row0 + first) : -1;
+  for (int64_t r = first; r < d.rows; r += step, R.parity ^= 1) {
+    float* row = d.row(r);
+    const int64_t t = next;
+    if (r + step < d.rows) next = id_at(d.tgt, d.tdt, d.row0 + r + step);
+    if (t < 0 || t >= d.V_) {
+      if (tid == 0) d.nll[d.row0 + r] = 0.0f;
+      for (int j = 0; j < R.chunks; ++j) {   // the copies must have left the row before it is written
+        R.wait(R.full_of(j), R.parity, 54);
+        R.release(j);
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory");
+      for (int g = tid; g < R.groups; g += nt) store_planes(row, d.ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      continue;
+    }
+    const float zt = tid == 0 ? row[t] : 0.0f;
+    const RowStat st = ring_stat(R, kLog2e, table, false);   // its barrier: the whole row has landed
+    if (tid == 0) d.nll[d.row0 + r] = logf(st.sum) - (zt - st.max);
+    const float f = 1.0f / st.sum;
+    ring_map(R, st, kLog2e, [&](int g, float4 e) {
+      float4 q = make_float4(e.x * f, e.y * f, e.z * f, e.w * f);
+      const unsigned o = (unsigned)((int)t - 4 * g);
+      if (o < 4) {
+        if (o == 0) q.x -= 1.0f;
+        if (o == 1) q.y -= 1.0f;
+        if (o == 2) q.z -= 1.0f;
+        if (o == 3) q.w -= 1.0f;
+      }
+      store_planes(row, d.ld, 4 * g, q);   // columns from V on hold exp(-inf) = 0
+    });
+  }
+}
+
+__device__ __forceinline__ void ring_rows(Ring& R, const Distill& d, float2* table, int64_t first, int64_t step) {
+  const int tid = (int)threadIdx.x, nt = R.chunk / 2, V = (int)d.V_;
+  const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T, inv_T = 1.0f / d.T;
+  // Entry k of a row is thread k's (and k + nt, ...); the first of them is fetched a row ahead.
+  Entry next = {-1, 0.0f, 0.0f, -1.0f};
+  int next_flag = 0;
+  if (first < d.rows) {
+    next_flag = d.flag[first];
+    if (tid < d.K) next = d.ent[first * d.K + tid];
+  }
+  for (int64_t r = first; r < d.rows; r += step, R.parity ^= 1) {
+    const float* row = d.row(r);
+    const RowSlice s = slice_of(row, V, 0, 0);
+    float* out = d.dl + r * d.V_;
+    float* part = d.part + r * d.parts;
+    const Entry mine = next;
+    const bool counted = next_flag;
+    if (r + step < d.rows) {
+      next_flag = d.flag[r + step];
+      if (tid < d.K) next = d.ent[(r + step) * d.K + tid];
+    }
+    if (!counted) {
+      if (tid < d.parts) part[tid] = 0.0f;
+      for (int j = 0; j < R.chunks; ++j) {
+        R.wait(R.full_of(j), R.parity, 54);
+        R.release(j);
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory");   // as every row: keeps the tables' turns
+      if (d.dl)
+        for (int e = tid; e < V; e += nt) out[e] = 0.0f;
+      continue;
+    }
+    const float z0 = mine.id >= 0 ? row[mine.id] : 0.0f;
+    const RowStat st = ring_stat(R, c, table, d.dl == nullptr);
+    if (d.dl) {
+      const bool vec = (((uintptr_t)out >> 2) & 3) == (unsigned)s.shift;
+      float4* base = reinterpret_cast<float4*>(out - s.shift);
+      const float f = scale / st.sum;
+      ring_map(R, st, c, [&](int g, float4 e) {
+        const float4 q = make_float4(e.x * f, e.y * f, e.z * f, e.w * f);
+        if (vec && g >= s.w0 && g < s.w1) base[g] = q;
+        else store_edge(out, V, 4 * g - s.shift, q);
+      });
+      asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory");   // the entries' columns are written again
+    }
+    if (tid < 32 * d.parts) {
+      const float ls = logf(st.sum);
+      float kl = 0.0f;
+      for (int k = tid; k < d.K; k += nt) {
+        const Entry e = k == tid ? mine : d.ent[r * d.K + k];
+        if (e.id < 0) continue;
+        const float z = k == tid ? z0 : row[e.id];
+        kl += entry_kl(e, z, st, ls, inv_T);
+        if (d.dl && e.own != -1.0f) out[e.id] = scale * (tc::exp2_hw((z - st.max) * c) / st.sum - e.own);
+      }
+      kl = wsum(kl);
+      if ((tid & 31) == 0) part[tid >> 5] = kl * (d.T * d.T);
+    }
+  }
+}
+
+template <class Op>
+__global__ void __launch_bounds__(32 * (kRingWarps + 1), 1) k_softmax_ring(const Op op, int groups) {
+  extern __shared__ __align__(16) float4 land[];
+  __shared__ uint64_t full[kRingChunks], empty[kRingChunks];
+  __shared__ float2 table[2 * kRingWarps];
+  const int warps = (int)(blockDim.x >> 5) - 1;
+  Ring R;
+  R.row = land;
+  R.full = tc::smem_u32(full);
+  R.empty = tc::smem_u32(empty);
+  R.chunk = 64 * warps;
+  R.chunks = (groups + R.chunk - 1) / R.chunk;
+  R.groups = groups;
+  R.parity = 0;
+  R.dead = false;
+  R.err = op.err;
+  if (threadIdx.x == 0) {
+    for (int j = 0; j < R.chunks; ++j) {
+      tc::mbar_init(R.full_of(j), 1);
+      tc::mbar_init(R.empty_of(j), (uint32_t)warps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if ((int)(threadIdx.x >> 5) == warps) ring_feed(R, op, blockIdx.x, gridDim.x);
+  else ring_rows(R, op, table, blockIdx.x, gridDim.x);
+}
+
+template <class Op>
+void launch_ring(const Op& op, int groups) {
+  const int warps = std::min(kRingWarps, (groups + 511) / 512);   // 16 groups a thread, or a little more
+  const size_t smem = (size_t)groups * 16;
+  static std::mutex mu;
+  static std::map<int, int> resident;   // blocks per SM, asked of the driver once per row length
+  static size_t most = 0;
+  std::lock_guard<std::mutex> lk(mu);
+  if (smem > most) {
+    MALUS_CUDA(cudaFuncSetAttribute(k_softmax_ring<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    most = smem;
+  }
+  int& res = resident[groups];
+  if (!res) {
+    MALUS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, k_softmax_ring<Op>, 32 * (warps + 1), smem));
+    if (res < 1) panic("softmax rows: no block of %d threads with %zu bytes can be resident", 32 * (warps + 1), smem);
+  }
+  const unsigned grid = (unsigned)std::min<int64_t>(op.rows, (int64_t)kNumSMs * res);
+  k_softmax_ring<Op><<<grid, 32 * (warps + 1), smem, stream()>>>(op, groups);
 }
 
 // Blocks per row and threads per block for rows of `groups` 16-byte groups;
@@ -701,6 +1005,8 @@ void xent_rows(float* logits, int64_t ld, int64_t n, int64_t V, const void* targ
   const int pid = prof_begin_named("k_xent_rows", 8.0 * (double)n * (double)ld);
   if (ld <= kShort)
     k_xent_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(logits, (int)ld, n, (int)V, targets, tgt_dtype, row0, nll);
+  else if (ld / 4 <= kRingGroups)
+    launch_ring(XentRows{logits, (int)ld, (int)V, n, targets, tgt_dtype, row0, nll, device_error_word()}, (int)(ld / 4));
   else if (!row_launch(ld / 4, &cs, &threads)) panic("softmax rows of %lld logits", (long long)V);
   else launch_rows(threads > kThreads ? k_xent_rows<kMaxThreads> : k_xent_rows<kThreads>, n, ld / 4, cs, threads, 0, logits, (int)ld, n, (int)V, targets, tgt_dtype, row0, nll, device_error_word());
   count_launch();
@@ -755,7 +1061,10 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   // a row may start 3 past an aligned address
   const int64_t groups = (V + 3 + 3) / 4;
   int cs = 1, threads = 0, parts = 1;
-  if (V > kShort) {
+  const bool ring = V > kShort && groups <= kRingGroups;
+  if (ring) {
+    parts = std::min((int)(K + 31) / 32, std::min(kRingWarps, (int)(groups + 511) / 512));
+  } else if (V > kShort) {
     if (!row_launch(groups, &cs, &threads)) panic("softmax rows of %lld logits", (long long)V);
     parts = cs * std::min((int)(K + 31) / 32, threads / 32);
   }
@@ -773,6 +1082,7 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
         idp, idt, te, n, (int)K, V, kLog2e / temperature, ent, flag, count, device_error_word());
     const int pid = prof_begin_named("k_distill_rows", (hd ? 8.0 : 4.0) * (double)n * (double)V);
     if (V <= kShort) k_distill_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(d);
+    else if (ring) launch_ring(d, (int)groups);
     else launch_rows(threads > kThreads ? k_distill_rows<kMaxThreads> : k_distill_rows<kThreads>, n, groups, cs, threads,
                      (size_t)K * 4, d);
     count_launch(2);
