@@ -287,7 +287,7 @@ void malus_layernorm_affine_bwd(int64_t x, int64_t weight, int64_t stats, int64_
  * gradient (a target at or past V is treated so too, and reported through
  * malus_device_error as 4).  Without counted rows the loss is 0.  dx and
  * dweight are the gradients of the loss (for dout = 1; see tape_record_loss).
- * V is limited to 262144. */
+ * V is limited to 2^24. */
 int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
                           int64_t* dweight);
 /* Distillation from a teacher's top logits: logits [N, V], and per row K <= 1024
@@ -297,7 +297,7 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
  * counted rows, those with an entry.  A negative id, or a teacher logit of
  * -inf, is no entry (an id at or past V is treated so too, and reported
  * through malus_device_error as 4); an id listed twice counts as both entries.
- * dlogits is the gradient of the loss (for dout = 1).  V is limited to 262140. */
+ * dlogits is the gradient of the loss (for dout = 1).  V is limited to 2^24. */
 int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temperature, int64_t* kl,
                       int64_t* dlogits);
 /* Tape records of the above.  stats, and the n gradients of a loss with respect

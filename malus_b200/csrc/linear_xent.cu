@@ -53,17 +53,19 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   if (dx && tied) f16_split_cols(w, V, D, wd.hi, wd.lo, wd.inv, nullptr, 0, 0);
   if (dx && !tied) f16_split_rows(w, D, V, wd.hi, wd.lo, wd.inv);
   // pieces of whole 256-row tiles, of even size
-  const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * 4)) / 256 * 256);
+  const bool in_place = xent_rows_in_place(ld);
+  const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8))) / 256 * 256);
   const int64_t pieces = (n + most - 1) / most;
   const int64_t piece = ((n + pieces - 1) / pieces + 255) / 256 * 256;
   float* logits = static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
-  const __half* hi = reinterpret_cast<const __half*>(logits);
+  float* planes = in_place ? logits : static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
+  const __half* hi = reinterpret_cast<const __half*>(planes);
   constexpr float inv = 1.0f / (1 << kF16Exp);
   for (int64_t r0 = 0; r0 < n; r0 += piece) {
     const int64_t m = std::min(piece, n - r0);
     F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), logits, ld, false, nullptr};
     gemm_f16(g);
-    xent_rows(logits, ld, m, V, tgt, tdt, r0, nll);
+    xent_rows(logits, planes, ld, m, V, tgt, tdt, r0, nll);
     if (dx) {
       const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, false, 0, nullptr, inv};
       gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, count});
@@ -75,6 +77,7 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
       else gemm_f16({(int)D, (int)V, (int)m, xt, dl, dw, V, r0 > 0, count});
     }
   }
+  if (!in_place) scratch_free(planes);
   scratch_free(logits);
 }
 

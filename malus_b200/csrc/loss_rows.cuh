@@ -12,11 +12,13 @@ void xent_count(const void* targets, int tgt_dtype, int64_t n, int64_t V, int* c
 
 // Rows [0, n) of f32 logits (row pitch ld >= V, a multiple of 64) against
 // targets[row0 ..]: nll[row0 + r] = logsumexp - logits[target] (0 for rows left
-// out), and the row's memory becomes the half planes of 2^kF16Exp (softmax -
-// onehot): hi in its first ld halves, lo in the next ld; zeros for rows left out
-// and for the columns from V to ld.
-void xent_rows(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, int64_t row0,
-               float* nll);
+// out), and the half planes of 2^kF16Exp (softmax - onehot): hi in the first ld
+// halves of row r of `planes` (pitch ld floats), lo in the next ld; zeros for rows
+// left out and for the columns from V to ld.  planes may be logits itself where
+// xent_rows_in_place(ld).
+bool xent_rows_in_place(int64_t ld);
+void xent_rows(const float* logits, float* planes, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype,
+               int64_t row0, float* nll);
 
 // nll[r] of n rows from the statistics of gemm_f16_lse
 void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,
@@ -25,6 +27,6 @@ void xent_join(const float2* part, int parts, const float* at, const void* targe
 // loss[0] = sum of v[0 .. n) / max(1, count[0])
 void loss_mean(float* v, int64_t n, const int* count, float* loss);
 
-constexpr int64_t kMaxRowLogits = 262144;   // longest row (pitch) xent_rows takes
+constexpr int64_t kMaxRowLogits = (int64_t)1 << 24;   // longest row
 
 }  // namespace malus

@@ -1,6 +1,6 @@
 """GPU: distillation from a teacher's top logits (malus_distill) against its
-formula in 64 bits: one block, clusters of blocks and the longest rows, aligned
-and not, ragged, repeated and missing entries, i32 and i64 ids, and the tape.
+formula in 64 bits: rows of a warp, rows that stay in a block's shared memory and
+longer ones, aligned and not, ragged, repeated and missing entries, i32 and i64 ids, and the tape.
 
 Tolerances (u = 2^-24): a base-2 exponential argument z = (s - max) * c carries
 3 roundings, so exp has a relative error of 3 u |z| + 4 u (exp2f is within two
@@ -74,7 +74,7 @@ def check(got, ref, tol, msg=""):
     (5, 1000, 64, 1.0, np.int32, 0.9), (4, 10007, 20, 3.0, np.int64, 0.2), (3, 16381, 7, 1.5, np.int32, 0.0),
     (3, 16384, 33, 1.0, np.int32, 0.0), (2, 16385, 33, 1.0, np.int32, 0.0), (5, 32003, 20, 1.0, np.int64, 0.3),
     (3, 50304, 64, 2.0, np.int32, 0.0), (2, 65537, 100, 1.0, np.int32, 0.1), (2, 140001, 1024, 2.0, np.int64, 0.1),
-    (1, 262140, 3, 1.0, np.int32, 0.0), (2000, 33, 4, 2.0, np.int32, 0.5)])
+    (3, 262143, 3, 1.0, np.int32, 0.0), (2, 57597, 9, 1.0, np.int32, 0.0), (301, 57603, 9, 1.0, np.int32, 0.3), (2000, 33, 4, 2.0, np.int32, 0.5)])
 def test_against_the_formula(M, N, V, K, T, idt, pad):
     s, ids, te = inputs(N, V, K, N + V + K, idt, pad)
     check(run(M, s, ids, te, T), *reference(s, ids, te, T), f"N {N} V {V} K {K}")
