@@ -158,6 +158,9 @@ void malus_tape_registry_lens(int64_t* leaves, int64_t* grads);
  * handle lives in HBM on the current device). */
 void* malus_tensor_data(int64_t h);
 int32_t malus_tensor_dtype(int64_t h);
+/* All of the above in one call: out = (data pointer, dtype, rank, shape...), 11
+ * words at most; returns the rank. */
+int32_t malus_tensor_describe(int64_t h, int64_t* out);
 /* Copy a tensor to / from host memory (synchronous). */
 void malus_tensor_read(int64_t h, void* dst, size_t bytes);
 void malus_tensor_write(int64_t h, const void* src, size_t bytes);

@@ -117,6 +117,7 @@ SIGNATURES: dict[str, tuple] = {
     "malus_tape_registry_lens": (None, [P_i64, P_i64]),
     "malus_tensor_data": (vp, [i64]),
     "malus_tensor_dtype": (i32, [i64]),
+    "malus_tensor_describe": (i32, [i64, P_i64]),
     "malus_tensor_read": (None, [i64, vp, sz]),
     "malus_tensor_write": (None, [i64, vp, sz]),
     "malus_tensor_wrap": (i64, [i32, vp, P_sz, sz]),
@@ -261,6 +262,11 @@ DTYPES = {np.dtype(np.float32): 0, np.dtype(np.int32): 5, np.dtype(np.int64): 6}
 NP_OF = {0: np.float32, 5: np.int32, 6: np.int64}
 
 
+_DTYPE_OF = {key: v for d, v in DTYPES.items() for key in (d, d.type, d.name)}
+_TYPESTR = {k: np.dtype(t).str for k, t in NP_OF.items()}
+_DESCRIBE = C.c_int64 * 11
+
+
 class Tensor:
     """Owning wrapper around a runtime handle (refcount released on close/del)."""
 
@@ -288,16 +294,18 @@ class Tensor:
         (malus_stream), until the work queued on it is done.  Work that another
         stream still has to do on the memory is the caller's to wait for."""
         s, n = _shape_arr(shape)
-        return Tensor(load().malus_tensor_wrap(DTYPES[np.dtype(dtype)], ptr, s, n))
+        return Tensor(load().malus_tensor_wrap(_DTYPE_OF[dtype], ptr, s, n))
 
     @property
     def __cuda_array_interface__(self) -> dict:
         """The data for another library on the same GPU, without a copy.  It is
         written on the runtime's stream: wait for that (gpu_barrier) before
         reading it on another, and keep this object alive meanwhile."""
-        lib = load()
-        return {"shape": self.shape, "typestr": np.dtype(self.dtype).str, "strides": None, "version": 2,
-                "data": (lib.malus_tensor_data(self.h) if 0 not in self.shape else 0, False)}
+        d = _DESCRIBE()
+        n = load().malus_tensor_describe(self.h, d)
+        shape = tuple(d[3:3 + n])
+        return {"shape": shape, "typestr": _TYPESTR[d[1]], "strides": None, "version": 2,
+                "data": (0 if 0 in shape else d[0], False)}
 
     @property
     def shape(self) -> tuple:

@@ -460,30 +460,50 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* _
   }
 }
 
+// Whether row r is kept; loaded beside the row, not before it.
 __device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, int64_t r) {
   if (!keep) return true;
   const int64_t t = dt == MALUS_I64 ? ((const int64_t*)keep)[r] : (int64_t)((const int32_t*)keep)[r];
   return t >= 0 && t < limit;
 }
 
-// bits[c] = largest finite magnitude of column c (as bits; zeroed before):
-// 32 columns x 8 rows per block, a slice of rows per blockIdx.y
+// bits[c] = largest finite magnitude of column c (as bits; zeroed before): 32 x W
+// columns per block, 8 warps on every eighth row, a slice of rows per blockIdx.y
+template <int W>
 __global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
                                                  uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
-  __shared__ uint32_t sh[8][32];
+  __shared__ uint32_t sh[8][32 * W];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  uint32_t m = 0;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * W;
+  uint32_t m[W] = {};
   if (c < C) {
-#pragma unroll 8
-    for (int64_t r = (int64_t)blockIdx.y * 8 + g; r < R; r += (int64_t)gridDim.y * 8)
-      if (kept(keep, kdt, limit, r)) m = max(m, finite_bits(src[r * C + c]));
+    const int64_t step = (int64_t)gridDim.y * 8;
+    int64_t r = (int64_t)blockIdx.y * 8 + g;
+    for (; r < R; r += 8 * step) {
+      float v[8][W];
+      bool k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t q = r + i * step < R ? r + i * step : r;   // past the end: the first one again
+        const float* p = src + q * C + c;
+        if constexpr (W == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(p);
+        else v[i][0] = *p;
+        k[i] = kept(keep, kdt, limit, q);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) m[j] = max(m[j], k[i] ? finite_bits(v[i][j]) : 0u);
+    }
   }
-  sh[g][lane] = m;
+#pragma unroll
+  for (int j = 0; j < W; ++j) sh[g][j * 32 + lane] = m[j];
   __syncthreads();
-  if (g == 0 && c < C) {
-    for (int i = 1; i < 8; ++i) m = max(m, sh[i][lane]);
-    atomicMax(bits + c, m);   // a maximum: the order does not matter
+  for (int i = threadIdx.x; i < 32 * W; i += 256) {
+    uint32_t a = 0;
+    for (int k = 0; k < 8; ++k) a = max(a, sh[k][i]);
+    const int64_t col = ((int64_t)blockIdx.x * 32 + (i & 31)) * W + (i >> 5);
+    if (col < C) atomicMax(bits + col, a);   // a maximum: the order does not matter
   }
 }
 
@@ -496,13 +516,19 @@ __global__ void __launch_bounds__(256) k_split_cols(const float* __restrict__ sr
   const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * 64;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const int64_t c = c0 + tx;
+  float v[16];
+  bool k[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t r = r0 + ty + 4 * i;
+    const bool in = r < R && c < C;
+    v[i] = in ? src[r * C + c] : 0.0f;
+    k[i] = in && kept(keep, kdt, limit, r);
+  }
   float up = 1.0f, iv = 1.0f;
   if (c < C) scale_for(bits[c], &up, &iv);
 #pragma unroll
-  for (int i = ty; i < 64; i += 4) {
-    const int64_t r = r0 + i;
-    tile[i][tx] = r < R && c < C && kept(keep, kdt, limit, r) ? src[r * C + c] * up : 0.0f;
-  }
+  for (int i = 0; i < 16; ++i) tile[ty + 4 * i][tx] = k[i] ? v[i] * up : 0.0f;
   if (blockIdx.y == 0 && ty == 0 && c < C) inv[c] = iv;
   __syncthreads();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -689,9 +715,11 @@ void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* 
   uint32_t* bits = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
   const int pid = prof_begin(1, 0.0, 8.0 * (double)R * (double)C);
   MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
-  const int64_t cb = (C + 31) / 32;
-  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 63) / 64, (kNumSMs * 16 + cb - 1) / cb));
-  k_col_max<<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
+  const int64_t cb = vec ? (C + 127) / 128 : (C + 31) / 32;
+  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 63) / 64, (kNumSMs * 8 + cb - 1) / cb));
+  if (vec) k_col_max<4><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  else k_col_max<1><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
   if (Rp / 64 > 65535) panic("f16_split_cols of %lld rows", (long long)R);
   k_split_cols<<<dim3((unsigned)((C + 63) / 64), (unsigned)(Rp / 64)), 256, 0, stream()>>>(
       src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);

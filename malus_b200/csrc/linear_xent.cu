@@ -12,7 +12,10 @@
 // loss alone stores no logits: the product's epilogue reduces each row of a tile
 // to its maximum, sum of exponentials and target logit.
 //
-// All products run as three half-precision ones (gemm_f16.cuh).  x and weight
+// The loss of a few rows (a token being scored) reads the weight once as it is, with
+// f32 multiply-adds: nothing is split, and that one read is what bounds it.
+//
+// All other products run as three half-precision ones (gemm_f16.cuh).  x and weight
 // are split twice, by rows and by columns, so that every product's operands are
 // scaled along the axis it does not sum over.
 #include "gemm_f16.cuh"
@@ -97,6 +100,247 @@ void loss_only(const void* tgt, int tdt, int64_t n, int64_t D, int64_t V, const 
   scratch_free(part);
 }
 
+// ------------------------------------------------------------- few rows
+constexpr int kFewRows = 8;
+constexpr int kFewSmem = 96 * 1024;   // x rows held in shared memory
+constexpr int kFewWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Running maximum and sum of exponentials.
+struct Run {
+  float m = -INFINITY, s = 0.0f;
+  __device__ __forceinline__ void add(float z) {
+    const float mn = fmaxf(m, z), m0 = mn == -INFINITY ? 0.0f : mn;
+    s = s * exp2f((m - m0) * kLog2e) + exp2f((z - m0) * kLog2e);
+    m = mn;
+  }
+  __device__ __forceinline__ void join(float om, float os) {
+    const float mn = fmaxf(m, om), m0 = mn == -INFINITY ? 0.0f : mn;
+    s = s * exp2f((m - m0) * kLog2e) + os * exp2f((om - m0) * kLog2e);
+    m = mn;
+  }
+};
+
+__device__ __forceinline__ int64_t target_at(const void* t, int dt, int64_t i) {
+  return dt == MALUS_I64 ? ((const int64_t*)t)[i] : (int64_t)((const int32_t*)t)[i];
+}
+
+// weight [V, D]: a warp takes four vocabulary entries at a time against all N rows
+// of x, its lanes along D.  The 4 N sums are reduced by halving: each exchange
+// leaves half as many to a lane, until every lane has one logit (or a share of
+// it), whose running softmax it keeps.  part: [N][gridDim.x].
+template <int N, bool VEC>
+__global__ void __launch_bounds__(32 * kFewWarps, N <= 2 ? 4 : 2)
+k_head_few_rows(const float* __restrict__ x, const float* __restrict__ w, int n, int D, int V, const void* tgt, int tdt,
+                float2* __restrict__ part, float* __restrict__ at) {
+  extern __shared__ __align__(16) float xs[];   // [N][Dp], zeros past n and D
+  __shared__ float2 sh[kFewWarps][4 * N];
+  const int Dp = (D + 127) / 128 * 128, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < N * Dp; i += blockDim.x) {
+    const int r = i / Dp, c = i % Dp;
+    xs[i] = r < n && c < D ? x[(int64_t)r * D + c] : 0.0f;
+  }
+  __syncthreads();
+  // which of the 4 N logits (entry j, row i at j * N + i) ends in this lane
+  int idx = 0, left = 4 * N;
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    if (left > 1) {
+      left /= 2;
+      if (lane & o) idx += left;
+    }
+  const int my_row = idx % N, my_entry = idx / N;
+  const int64_t t = my_row < n ? target_at(tgt, tdt, my_row) : -1;
+  Run run;
+  const int step = (int)gridDim.x * kFewWarps * 4;
+  for (int v0 = ((int)blockIdx.x * kFewWarps + warp) * 4; v0 < V; v0 += step) {
+    float a[4 * N];
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) a[i] = 0.0f;
+#pragma unroll 2
+    for (int c = 0; c < Dp; c += 128) {
+      float4 q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* p = w + (int64_t)min(v0 + j, V - 1) * D;
+        if (VEC) {
+          const int e = c + 4 * lane;
+          q[j] = e < D ? *reinterpret_cast<const float4*>(p + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          const int e = c + lane;
+          q[j] = make_float4(e < D ? p[e] : 0.f, e + 32 < D ? p[e + 32] : 0.f, e + 64 < D ? p[e + 64] : 0.f,
+                             e + 96 < D ? p[e + 96] : 0.f);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float* p = xs + i * Dp + c;
+        const float4 u = VEC ? *reinterpret_cast<const float4*>(p + 4 * lane)
+                             : make_float4(p[lane], p[lane + 32], p[lane + 64], p[lane + 96]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          a[j * N + i] = fmaf(q[j].x, u.x, fmaf(q[j].y, u.y, fmaf(q[j].z, u.z, fmaf(q[j].w, u.w, a[j * N + i]))));
+      }
+    }
+    int cnt = 4 * N;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      if (cnt > 1) {
+        cnt /= 2;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i)
+          if (i < cnt) {
+            const float give = lane & o ? a[i] : a[i + cnt], keep = lane & o ? a[i + cnt] : a[i];
+            a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+      } else {
+        a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+      }
+    }
+    const int v = v0 + my_entry;
+    if (v < V) {
+      run.add(a[0]);
+      if (v == t) at[my_row] = a[0];   // the lanes of a logit write the same value
+    }
+  }
+  sh[warp][idx] = make_float2(run.m, run.s);
+  __syncthreads();
+  if (threadIdx.x < n) {
+    Run r;
+    for (int k = 0; k < kFewWarps; ++k)
+      for (int j = 0; j < 4; ++j) r.join(sh[k][j * N + threadIdx.x].x, sh[k][j * N + threadIdx.x].y);
+    part[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(r.m, r.s);
+  }
+}
+
+// weight [D, V]: a block takes 32 W columns, its warps a slice of D each, and joins
+// their sums through shared memory.  part: [N][gridDim.x].
+template <int N, int W>
+__global__ void __launch_bounds__(32 * kFewWarps, 3)
+k_head_few_cols(const float* __restrict__ x, const float* __restrict__ w, int n, int D, int V, const void* tgt, int tdt,
+                float2* __restrict__ part, float* __restrict__ at) {
+  extern __shared__ __align__(16) float xs[];   // [D][N], then [warps][N][32 W]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* sums = xs + (int64_t)D * N;
+  for (int i = threadIdx.x; i < N * D; i += blockDim.x) xs[i] = i % N < n ? x[(int64_t)(i % N) * D + i / N] : 0.0f;
+  __syncthreads();
+  const int c = ((int)blockIdx.x * 32 + lane) * W;
+  const int d0 = (int)((int64_t)D * warp / kFewWarps), d1 = (int)((int64_t)D * (warp + 1) / kFewWarps);
+  float a[N][W];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) a[i][j] = 0.0f;
+  if (c < V) {
+    for (int d = d0; d < d1; d += 8) {
+      float q[8][W];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float* p = w + (int64_t)min(d + k, d1 - 1) * V + c;
+        if constexpr (W == 4) *reinterpret_cast<float4*>(q[k]) = *reinterpret_cast<const float4*>(p);
+        else q[k][0] = *p;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (d + k < d1)
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float u = xs[(d + k) * N + i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) a[i][j] = fmaf(q[k][j], u, a[i][j]);
+          }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) sums[(warp * N + i) * 32 * W + lane * W + j] = a[i][j];
+  __syncthreads();
+  // a warp per row: logits of the block's columns, their running softmax
+  for (int i = warp; i < n; i += kFewWarps) {
+    const int64_t t = target_at(tgt, tdt, i);
+    Run r;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int col = j * 32 + lane, v = (int)blockIdx.x * 32 * W + col;
+      float z = 0.0f;
+      for (int k = 0; k < kFewWarps; ++k) z += sums[(k * N + i) * 32 * W + col];
+      if (v < V) {
+        r.add(z);
+        if (v == t) at[i] = z;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      r.join(__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o));
+    if (lane == 0) part[(int64_t)i * gridDim.x + blockIdx.x] = make_float2(r.m, r.s);
+  }
+}
+
+// The rows' nll from their parts and the loss, in one block: a warp per row.
+__global__ void __launch_bounds__(32 * kFewRows)
+k_head_few_end(const float2* __restrict__ part, int parts, const float* __restrict__ at, const void* tgt, int tdt, int n,
+               int V, float* __restrict__ nll, float* __restrict__ loss, int32_t* __restrict__ err) {
+  __shared__ float sh[kFewRows];
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5;
+  float v = 0.0f;
+  bool counted = false;
+  if (i < n) {
+    const int64_t t = target_at(tgt, tdt, i);
+    counted = t >= 0 && t < V;
+    if (t >= V && lane == 0) atomicExch(err, 4);
+    Run r;
+    for (int k = lane; k < parts; k += 32) {
+      const float2 o = part[(int64_t)i * parts + k];
+      r.join(o.x, o.y);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      r.join(__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o));
+    if (counted) v = logf(r.s) - (at[i] - r.m);
+    if (lane == 0) nll[i] = v;
+  }
+  if (lane == 0) sh[i] = v;
+  const int count = __syncthreads_count(counted && lane == 0);
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int k = 0; k < kFewRows; ++k) s += (double)sh[k];
+    loss[0] = (float)(s / (double)max(1, count));
+  }
+}
+
+template <int N>
+void few(const float* x, const float* w, const void* tgt, int tdt, bool tied, int n, int D, int V, float* nll,
+         float* loss) {
+  // tied: two blocks' worth of warps per SM and more, as the registers allow; else a block per 32 or 128 columns
+  const bool vec = (tied ? D : V) % 4 == 0 && ((uintptr_t)w & 15) == 0;
+  const int grid = tied ? std::min((V + 4 * kFewWarps - 1) / (4 * kFewWarps), kNumSMs * 4)
+                        : (V + (vec ? 127 : 31)) / (vec ? 128 : 32);
+  float2* part = static_cast<float2*>(scratch_alloc((size_t)n * (grid * 8 + 4)));
+  float* at = reinterpret_cast<float*>(part + (int64_t)n * grid);
+  const int pid = prof_begin_named("k_head_few", 4.0 * (double)V * D);
+  auto go = [&](auto kernel, size_t smem) {
+    MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<grid, 32 * kFewWarps, smem, stream()>>>(x, w, n, D, V, tgt, tdt, part, at);
+  };
+  const size_t rows = (size_t)N * ((D + 127) / 128 * 128) * 4;
+  const size_t cols = (size_t)N * (D + kFewWarps * (vec ? 128 : 32)) * 4;
+  if (tied) vec ? go(k_head_few_rows<N, true>, rows) : go(k_head_few_rows<N, false>, rows);
+  else vec ? go(k_head_few_cols<N, 4>, cols) : go(k_head_few_cols<N, 1>, cols);
+  prof_end(pid);
+  k_head_few_end<<<1, 32 * kFewRows, 0, stream()>>>(part, grid, at, tgt, tdt, n, V, nll, loss, device_error_word());
+  count_launch(2);
+  after_launch("k_head_few");
+  scratch_free(part);
+}
+
+// Rows that take this path: x in shared memory beside the block's sums.
+bool few_rows(int64_t n, int64_t D) {
+  if (n < 1 || n > kFewRows) return false;
+  const int64_t N = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+  return N * (D + 127 + kFewWarps * 128) * 4 <= kFewSmem;
+}
+
 }  // namespace
 }  // namespace malus
 
@@ -127,6 +371,15 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
   const void* tp = vptr(targets);
   const int64_t loss = alloc_f32({1}), hn = alloc_f32({n});
   const int64_t hx = dx ? alloc_shape(sx) : 0, hw = dweight ? alloc_shape(sw) : 0;
+  if (!hx && !hw && few_rows((int64_t)n, (int64_t)D)) {
+    auto go = n <= 1 ? few<1> : n <= 2 ? few<2> : n <= 4 ? few<4> : few<8>;
+    go(xp, wp, tp, tdt, tied != 0, (int)n, (int)D, (int)V, fptr(hn), fptr(loss));
+    if (nll) *nll = hn;
+    else tensor_release(hn);
+    if (dx) *dx = 0;
+    if (dweight) *dweight = 0;
+    return loss;
+  }
   int* count = static_cast<int*>(scratch_alloc(4));
   xent_count(tp, tdt, (int64_t)n, (int64_t)V, count);
   if (n == 0) {

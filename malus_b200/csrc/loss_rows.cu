@@ -185,10 +185,15 @@ __global__ void __launch_bounds__(1024) k_xent_count(const void* __restrict__ tg
   __shared__ int sh[32];
   int c = 0;
   bool bad = false;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-    const int64_t t = id_at(tgt, tdt, i);
-    c += t >= 0 && t < V;
-    bad |= t >= V;
+  for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+    int64_t t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = i + k * 1024 < n ? id_at(tgt, tdt, i + k * 1024) : -1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      c += t[k] >= 0 && t[k] < V;
+      bad |= t[k] >= V;
+    }
   }
   if (bad) atomicExch(err, kErrId);
 #pragma unroll

@@ -200,27 +200,33 @@ k_norm_bwd(const float* __restrict__ x, const float* __restrict__ w, const float
   }
 }
 
-// out[c] = sum over the nb partial rows, in order within each of the 8 groups
-// of rows and then over the groups.
-__global__ void __launch_bounds__(256) k_norm_fold(const float* __restrict__ part, int nb, int D,
-                                                   float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float sh[8][33];
+// out[c] = sum over the nb partial rows, in order within each of the 32 groups of
+// rows and then over the groups.
+__global__ void __launch_bounds__(1024) k_norm_fold(const float* __restrict__ part, int nb, int D,
+                                                    float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;   // column of the [2 * D] partial row
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane, W = 2 * (int64_t)D;   // column of the partial row
   float s = 0.0f;
-  if (c < 2 * (int64_t)D) {
-    const int per = (nb + 7) / 8, lo = g * per, hi = min(nb, lo + per);
-#pragma unroll 8
-    for (int i = lo; i < hi; ++i) s += part[(int64_t)i * 2 * D + c];
+  if (c < W) {
+    const int per = (nb + 31) / 32, lo = g * per, hi = min(nb, lo + per);
+    for (int i = lo; i < hi; i += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i + k < hi ? part[(int64_t)(i + k) * W + c] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
   }
   sh[g][lane] = s;
   __syncthreads();
-  if (g == 0 && c < 2 * (int64_t)D) {
-    s = 0.0f;
+  s = sh[lane][g];   // group `lane` of column g
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += sh[i][lane];
-    float* out = c < D ? dw : db;
-    if (out) out[c < D ? c : c - D] = s;
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t col = (int64_t)blockIdx.x * 32 + g;
+  if (lane == 0 && col < W) {
+    float* out = col < D ? dw : db;
+    if (out) out[col < D ? col : col - D] = s;
   }
 }
 
@@ -365,7 +371,7 @@ struct BwdLaunch {
     float* part = cols ? static_cast<float*>(scratch_alloc((size_t)grid * 2 * D * 4)) : nullptr;
     k_norm_bwd<TPR, NV, VEC><<<grid, BLOCK, smem, stream()>>>(x, w, stats, dy, dx, part, rows, D);
     if (cols) {
-      k_norm_fold<<<(2 * D + 31) / 32, 256, 0, stream()>>>(part, grid, D, dw, db);
+      k_norm_fold<<<(2 * D + 31) / 32, 1024, 0, stream()>>>(part, grid, D, dw, db);
       count_launch();
       scratch_free(part);
     }
@@ -410,7 +416,7 @@ void norm_affine_bwd(const float* x, const float* w, const float* stats, const f
       const int nb = (int)std::min<int64_t>(rows, 32);
       float* part = static_cast<float*>(scratch_alloc((size_t)nb * 2 * D * 4));
       k_norm_dw_long<<<dim3((unsigned)((D + 255) / 256), nb), 256, 0, stream()>>>(x, stats, dy, part, rows, D);
-      k_norm_fold<<<(unsigned)((2 * D + 31) / 32), 256, 0, stream()>>>(part, nb, (int)D, dw, db);
+      k_norm_fold<<<(unsigned)((2 * D + 31) / 32), 1024, 0, stream()>>>(part, nb, (int)D, dw, db);
       count_launch(2);
       scratch_free(part);
     }

@@ -909,6 +909,14 @@ void* malus_tensor_data(int64_t h) {
   return vptr(h);
 }
 int32_t malus_tensor_dtype(int64_t h) { return tb(h)->dtype; }
+int32_t malus_tensor_describe(int64_t h, int64_t* out) {
+  const auto* t = tb(h);
+  out[0] = reinterpret_cast<int64_t>(malus_tensor_data(h));
+  out[1] = t->dtype;
+  out[2] = t->ndim;
+  for (int i = 0; i < t->ndim; ++i) out[3 + i] = (int64_t)t->shape[i];
+  return t->ndim;
+}
 void malus_tensor_read(int64_t h, void* dst, size_t bytes) {
   auto* t = tb(h);
   size_t have = t->len * dtype_size(t->dtype);

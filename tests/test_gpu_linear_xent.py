@@ -78,7 +78,7 @@ def check(got, ref, tol, msg=""):
         assert not bad.any(), f"{what} {msg}: {bad.sum()} of {bad.size} off, worst {np.max(np.abs(g - r) / (t + 1e-36)):.3g}"
 
 
-SIZES = [(1, 1, 1), (1, 64, 50), (3, 5, 2), (7, 33, 65), (64, 64, 64), (65, 63, 129), (128, 128, 256), (129, 130, 257),
+SIZES = [(1, 1, 1), (1, 64, 50), (1, 700, 9001), (4, 129, 300), (8, 384, 1000), (3, 5, 2), (7, 33, 65), (64, 64, 64), (65, 63, 129), (128, 128, 256), (129, 130, 257),
          (256, 256, 256), (257, 65, 511), (300, 500, 1007), (511, 257, 300), (1000, 384, 65), (2, 768, 4099),
          (700, 96, 4096), (40, 16, 70001), (9, 24, 131200)]
 
