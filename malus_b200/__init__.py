@@ -329,7 +329,8 @@ class Tensor:
 
     def __del__(self):
         try:
-            self.close()
+            if self._owned and self.h:
+                _lib.tensor_release(self.h)
         except Exception:
             pass
 

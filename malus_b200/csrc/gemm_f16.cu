@@ -468,18 +468,17 @@ __device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, in
 }
 
 // bits[c] = largest finite magnitude of column c (as bits; zeroed before): 32 x W
-// columns per block, 8 warps on every eighth row, a slice of rows per blockIdx.y
+// columns per block, 32 warps on every 32nd row, a slice of rows per blockIdx.y
 template <int W>
-__global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
-                                                 uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
-  __shared__ uint32_t sh[8][32 * W];
+__global__ void __launch_bounds__(1024) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
+                                                  uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
+  __shared__ uint32_t sh[32][32 * W];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * W;
   uint32_t m[W] = {};
   if (c < C) {
-    const int64_t step = (int64_t)gridDim.y * 8;
-    int64_t r = (int64_t)blockIdx.y * 8 + g;
-    for (; r < R; r += 8 * step) {
+    const int64_t step = (int64_t)gridDim.y * 32;
+    for (int64_t r = (int64_t)blockIdx.y * 32 + g; r < R; r += 8 * step) {
       float v[8][W];
       bool k[8];
 #pragma unroll
@@ -499,48 +498,68 @@ __global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, 
 #pragma unroll
   for (int j = 0; j < W; ++j) sh[g][j * 32 + lane] = m[j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * W; i += 256) {
-    uint32_t a = 0;
-    for (int k = 0; k < 8; ++k) a = max(a, sh[k][i]);
+  // warp g takes W of the columns: its lanes the 32 warps' maxima
+  for (int i = g; i < 32 * W; i += 32) {
+    const uint32_t a = __reduce_max_sync(0xffffffffu, sh[lane][i]);
     const int64_t col = ((int64_t)blockIdx.x * 32 + (i & 31)) * W + (i >> 5);
-    if (col < C) atomicMax(bits + col, a);   // a maximum: the order does not matter
+    if (lane == 0 && col < C) atomicMax(bits + col, a);   // a maximum: the order does not matter
   }
 }
 
-// 64 x 64 tiles through shared memory: rows of the source in, columns out.
+// 64 x 64 tiles through shared memory: rows of the source in (16-byte groups when
+// VEC), columns out, 4 rows (8 bytes of a plane) per lane.
+template <bool VEC>
 __global__ void __launch_bounds__(256) k_split_cols(const float* __restrict__ src, int64_t R, int64_t C, int64_t Rp,
                                                     const uint32_t* __restrict__ bits, __half* __restrict__ hi,
                                                     __half* __restrict__ lo, float* __restrict__ inv, const void* keep,
                                                     int kdt, int64_t limit) {
   __shared__ float tile[64][65];
+  __shared__ float ups[64];
+  __shared__ uint32_t rows_kept[2];
   const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int64_t c = c0 + tx;
+  const int nr = (int)min((int64_t)64, R - r0), nc = (int)min((int64_t)64, C - c0), t = threadIdx.x;   // nr may be < 0
+  const float* p = src + r0 * C + c0;
+  constexpr int kStep = VEC ? 16 : 4;                     // rows between a thread's
+  const int tx = VEC ? (t & 15) * 4 : t & 63, ty = VEC ? t >> 4 : t >> 6;
   float v[16];
-  bool k[16];
+  if (VEC) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = r0 + ty + 4 * i;
-    const bool in = r < R && c < C;
-    v[i] = in ? src[r * C + c] : 0.0f;
-    k[i] = in && kept(keep, kdt, limit, r);
+    for (int i = 0; i < 4; ++i) {
+      const float4 q = ty + 16 * i < nr && tx < nc ? *reinterpret_cast<const float4*>(p + (int64_t)(ty + 16 * i) * C + tx)
+                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    }
+  } else {
+    const float* q = p + (int64_t)ty * C + tx;
+#pragma unroll
+    for (int i = 0; i < 16; ++i, q += 4 * C) v[i] = ty + 4 * i < nr && tx < nc ? *q : 0.0f;
   }
-  float up = 1.0f, iv = 1.0f;
-  if (c < C) scale_for(bits[c], &up, &iv);
+  if (t < 64) {
+    const bool k = t < nr && kept(keep, kdt, limit, r0 + t);
+    const uint32_t b = __ballot_sync(0xffffffffu, k);
+    if ((t & 31) == 0) rows_kept[t >> 5] = b;
+    float up = 1.0f, iv = 1.0f;
+    if (t < nc) scale_for(bits[c0 + t], &up, &iv);
+    ups[t] = up;
+    if (blockIdx.y == 0 && t < nc) inv[c0 + t] = iv;
+  }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) tile[ty + 4 * i][tx] = k[i] ? v[i] * up : 0.0f;
-  if (blockIdx.y == 0 && ty == 0 && c < C) inv[c] = iv;
+  for (int i = 0; i < 16; ++i) tile[ty + kStep * (VEC ? i >> 2 : i)][tx + (VEC ? i & 3 : 0)] = v[i];
   __syncthreads();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int r = (t & 15) * 4;
+  const uint32_t k4 = rows_kept[r >> 5] >> (r & 31);
+  __half* h0 = hi + c0 * Rp + r0 + r;
+  __half* l0 = lo + c0 * Rp + r0 + r;
 #pragma unroll
-  for (int i = w; i < 64; i += 8) {
-    if (c0 + i >= C) continue;
-    __align__(4) __half h[2], l[2];
-    split2(tile[2 * lane][i], &h[0], &l[0]);
-    split2(tile[2 * lane + 1][i], &h[1], &l[1]);
-    const int64_t o = (c0 + i) * Rp + r0 + 2 * lane;
-    *reinterpret_cast<uint32_t*>(hi + o) = *reinterpret_cast<uint32_t*>(h);
-    *reinterpret_cast<uint32_t*>(lo + o) = *reinterpret_cast<uint32_t*>(l);
+  for (int i = 0; i < 4; ++i) {
+    const int c = (t >> 4) + 16 * i;
+    if (c >= nc) break;
+    const float up = ups[c];
+    __align__(8) __half h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split2(k4 >> k & 1 ? tile[r + k][c] * up : 0.0f, &h[k], &l[k]);
+    *reinterpret_cast<uint2*>(h0 + c * Rp) = *reinterpret_cast<uint2*>(h);
+    *reinterpret_cast<uint2*>(l0 + c * Rp) = *reinterpret_cast<uint2*>(l);
   }
 }
 
@@ -717,12 +736,14 @@ void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* 
   MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
   const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
   const int64_t cb = vec ? (C + 127) / 128 : (C + 31) / 32;
-  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 63) / 64, (kNumSMs * 8 + cb - 1) / cb));
-  if (vec) k_col_max<4><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
-  else k_col_max<1><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  // few slices: their maxima meet in one word per column
+  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 255) / 256, (kNumSMs * 2 + cb - 1) / cb));
+  if (vec) k_col_max<4><<<dim3((unsigned)cb, ry), 1024, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  else k_col_max<1><<<dim3((unsigned)cb, ry), 1024, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
   if (Rp / 64 > 65535) panic("f16_split_cols of %lld rows", (long long)R);
-  k_split_cols<<<dim3((unsigned)((C + 63) / 64), (unsigned)(Rp / 64)), 256, 0, stream()>>>(
-      src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
+  const dim3 grid((unsigned)((C + 63) / 64), (unsigned)(Rp / 64));
+  if (vec) k_split_cols<true><<<grid, 256, 0, stream()>>>(src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
+  else k_split_cols<false><<<grid, 256, 0, stream()>>>(src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
   count_launch(2);
   after_launch("k_split_cols");
   scratch_free(bits);

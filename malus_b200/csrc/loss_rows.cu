@@ -26,7 +26,7 @@
 namespace malus {
 namespace {
 
-constexpr int kNV = 8;            // float4 groups a lane holds of a short row
+constexpr int kNV = 8;            // float4 groups a lane holds of a short row, at most
 constexpr int kMaxEntries = 1024; // teacher entries of a row
 constexpr int kShort = 32 * kNV * 4 - 4;   // longest row of a warp (it may start 3 past a 16-byte group)
 constexpr int kWarps = 8;         // rows per block of the short-row kernels
@@ -85,15 +85,16 @@ struct RowStat { float max, sum; };
 // Of a row held by one warp in v (-inf where a lane has no group); v becomes the
 // exponentials.  The exponential is the hardware's base-2 one (relative error
 // 2^-22; results below 2^-126 are 0).
-__device__ __forceinline__ RowStat warp_stat(float4 (&v)[kNV], float c) {
+template <int NV>
+__device__ __forceinline__ RowStat warp_stat(float4 (&v)[NV], float c) {
   float m = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kNV; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+  for (int k = 0; k < NV; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
   m = wmax(m);
   const float m0 = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kNV; ++k) {
+  for (int k = 0; k < NV; ++k) {
     v[k].x = tc::exp2_hw((v[k].x - m0) * c);
     v[k].y = tc::exp2_hw((v[k].y - m0) * c);
     v[k].z = tc::exp2_hw((v[k].z - m0) * c);
@@ -150,6 +151,7 @@ struct XentRows {
   __device__ __forceinline__ int V() const { return V_; }       // logits among them
 };
 
+template <int NV>
 __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d) {
   const int lane = threadIdx.x & 31, ld = d.ld, V = d.V_;
   for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < d.rows; r += (int64_t)gridDim.x * kWarps) {
@@ -162,9 +164,9 @@ __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d
       continue;
     }
     const float zt = row[t];
-    float4 v[kNV];
+    float4 v[NV];
 #pragma unroll
-    for (int k = 0; k < kNV; ++k) {
+    for (int k = 0; k < NV; ++k) {
       const int e = 4 * (k * 32 + lane);
       v[k] = e + 4 <= V ? *reinterpret_cast<const float4*>(row + e) : load_edge(row, V, e);
     }
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d
     if (lane == 0) d.nll[d.row0 + r] = logf(st.sum) - (zt - st.max);
     const float f = 1.0f / st.sum;
 #pragma unroll
-    for (int k = 0; k < kNV; ++k) {
+    for (int k = 0; k < NV; ++k) {
       const int e = 4 * (k * 32 + lane);
       if (e < ld)   // columns from V on hold exp(-inf) = 0
         store_planes(out, ld, e, less_hot(make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f), (int)t, e));
@@ -212,13 +214,22 @@ __global__ void __launch_bounds__(1024) k_loss_mean(float* __restrict__ v, const
                                                     int64_t n, const int* __restrict__ count, float* __restrict__ loss) {
   __shared__ double sh[32];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-    if (parts) {
+  if (parts) {
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
       float a = 0.0f;
+#pragma unroll 8
       for (int j = 0; j < parts; ++j) a += part[i * parts + j];
       v[i] = a;
+      s += (double)a;
     }
-    s += (double)v[i];
+  } else {
+    for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+      float a[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = i + k * 1024 < n ? v[i + k * 1024] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += (double)a[k];
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -275,10 +286,11 @@ __global__ void __launch_bounds__(256)
 k_teacher(const void* __restrict__ ids, int idt, const float* __restrict__ teacher, int64_t n, int K, int64_t V,
           float c, Entry* __restrict__ ent, int* __restrict__ flag, int* __restrict__ count,
           int32_t* __restrict__ err) {
-  extern __shared__ int sid[];   // [8][K]: the rows' ids, -1 where there is no entry
+  extern __shared__ int sid[];   // [8][2][K]: the rows' ids (-1: no entry) and p
   __shared__ int sh[8];
   const int lane = threadIdx.x & 31;
-  int* mine = sid + (threadIdx.x >> 5) * K;
+  int* mine = sid + (threadIdx.x >> 5) * 2 * K;
+  float* ps = reinterpret_cast<float*>(mine + K);
   int rows = 0;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += (int64_t)gridDim.x * 8) {
     const int64_t o = r * K;
@@ -290,6 +302,7 @@ k_teacher(const void* __restrict__ ids, int idt, const float* __restrict__ teach
       bad |= id >= V;
       const bool there = entry_there(id, te, V);
       mine[k] = there ? (int)id : -1;
+      ps[k] = te;
       if (there) {
         m = fmaxf(m, te);
         any = true;
@@ -299,32 +312,27 @@ k_teacher(const void* __restrict__ ids, int idt, const float* __restrict__ teach
     m = wmax(m);
     any = __any_sync(0xffffffffu, any);
     float s = 0.0f;
-    for (int k = lane; k < K; k += 32) {
-      const float z = (teacher[o + k] - m) * c;   // base-2 units
-      const float e = mine[k] >= 0 ? exp2f(z) : 0.0f;
-      ent[o + k] = {mine[k], e, z * kLn2, -1.0f};
-      s += e;
-    }
+    for (int k = lane; k < K; k += 32)
+      if (mine[k] >= 0) s += exp2f((ps[k] - m) * c);
     s = wsum(s);
     const float ls = logf(s);
-    for (int k = lane; k < K; k += 32) {
-      ent[o + k].lp -= ls;
-      ent[o + k].p = ent[o + k].p == 0.0f ? 0.0f : ent[o + k].p / s;
-    }
-    __syncwarp();   // the other lanes' ids and p
+    __syncwarp();   // the other lanes' ids
     for (int k = lane; k < K; k += 32) {
       const int id = mine[k];
-      if (id < 0) continue;
-      float sum = ent[o + k].p;
-      for (int j = 0; j < K; ++j)
-        if (mine[j] == id && j != k) {
-          if (j < k) {
-            sum = -1.0f;
-            break;
+      const float z = (ps[k] - m) * c;   // base-2 units
+      float sum = id >= 0 ? exp2f(z) / s : -1.0f;
+      const float p = id >= 0 ? sum : 0.0f;
+      if (id >= 0)
+#pragma unroll 8
+        for (int j = 0; j < K; ++j)
+          if (mine[j] == id && j != k) {
+            if (j < k) {
+              sum = -1.0f;
+              break;
+            }
+            sum += exp2f((ps[j] - m) * c) / s;
           }
-          sum += ent[o + j].p;
-        }
-      ent[o + k].own = sum;
+      ent[o + k] = {id, p, z * kLn2 - ls, sum};
     }
     __syncwarp();   // the ids are rewritten by the next row
     if (lane == 0) flag[r] = any;
@@ -359,6 +367,7 @@ __device__ __forceinline__ float entry_kl(const Entry& e, float z, RowStat st, f
   return e.p != 0.0f ? e.p * (e.lp - ((z - st.max) * inv_T - log_sum)) : 0.0f;
 }
 
+template <int NV>
 __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill d) {
   const int lane = threadIdx.x & 31, V = (int)d.V_;
   const float scale = d.dl ? d.T / (float)max(1, *d.count) : 0.0f, c = kLog2e / d.T;
@@ -373,9 +382,9 @@ __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill
         for (int e = lane; e < V; e += 32) out[e] = 0.0f;
       continue;
     }
-    float4 v[kNV];
+    float4 v[NV];
 #pragma unroll
-    for (int k = 0; k < kNV; ++k) {
+    for (int k = 0; k < NV; ++k) {
       const int g = k * 32 + lane;
       v[k] = g >= sl.w0 && g < sl.w1 ? sl.base[g] : load_edge(row, V, 4 * g - sl.shift);
     }
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_distill_rows_warp(const Distill
       const float f = scale / st.sum;
       float4* base = reinterpret_cast<float4*>(out - sl.shift);
 #pragma unroll
-      for (int k = 0; k < kNV; ++k) {
+      for (int k = 0; k < NV; ++k) {
         const int g = k * 32 + lane;
         const float4 q = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
         if (vec && g >= sl.w0 && g < sl.w1) base[g] = q;
@@ -459,23 +468,38 @@ struct Ring {
   }
 };
 
-// The feeding warp: rows first, first + step, ... below rows.
+// The feeding warp: rows first, first + step, ... below rows.  At most 32 groups
+// follow a row's whole ones: its pitch is less than 64 elements longer, or its
+// alignment adds one.
 template <class R_, class Op>
 __device__ __forceinline__ void ring_feed(R_& R, const Op& op, int64_t first, int64_t step) {
   const int lane = threadIdx.x & 31;
+  // groups that are not four logits of the row are written by element, -inf past
+  // its end: the first (lane 0) and those from w1 on (one per lane); they are
+  // fetched a row ahead
+  auto w1_of = [&](const RowView& v) { return (op.V() + v.shift) >> 2; };   // whole groups of logits end here
+  RowView s, ns;
+  float4 head, tail, nhead, ntail;
+  auto fetch = [&](int64_t r) {
+    ns = view_row(op.row(r), op.width());
+    if (lane == 0 && ns.w0) nhead = load_edge(op.row(r), op.V(), -ns.shift);
+    ntail = load_edge(op.row(r), op.V(), 4 * (w1_of(ns) + lane) - ns.shift);
+  };
+  if (first < op.rows) fetch(first);
   for (int64_t r = first; r < op.rows && !R.dead; r += step, R.row_done()) {
-    const float* row = op.row(r);
-    const RowView s = view_row(row, op.width());
-    const int w1 = (op.V() + s.shift) >> 2;   // whole groups of logits end here
+    s = ns;
+    head = nhead;
+    tail = ntail;
+    if (r + step < op.rows) fetch(r + step);
+    const int w1 = w1_of(s);
     for (int j = 0; j < (R_::STAY ? 1 : 2) * R.chunks; ++j, R.step()) {
       const int slot = R.at(j);
       if (R.round && !R.dead) R.dead = !wait_for(R.empty_of(slot), (R.round - 1) & 1, R.err, 53);
       if (R.dead) break;
       const int lo = (j < R.chunks ? j : j - R.chunks) * R.chunk, hi = min(lo + R.chunk, R.groups);
       float4* at = R.buf + slot * R.chunk - lo;
-      // groups that are not four logits of the row: written by element, -inf past its end
-      if (lane == 0 && lo == 0 && s.w0) at[0] = load_edge(row, op.V(), -s.shift);
-      for (int g = max(lo, w1) + lane; g < hi; g += 32) at[g] = load_edge(row, op.V(), 4 * g - s.shift);
+      if (lane == 0 && lo == 0 && s.w0) at[0] = head;
+      if (w1 + lane >= lo && w1 + lane < hi) at[w1 + lane] = tail;
       __syncwarp();
       if (lane == 0) {
         const int i0 = max(lo, s.w0), i1 = min(hi, w1);
@@ -713,9 +737,26 @@ void launch_ring(const Op& op, int groups) {
   else launch_ring<false>(op, groups);
 }
 
-unsigned warp_row_blocks(int64_t rows) {
-  return (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, kNumSMs * 4);
+// Short rows: f(number of float4 groups a lane holds, as a constant; blocks).
+template <class F>
+void with_warp_rows(int64_t groups, int64_t rows, F&& f) {
+  const int nv = (int)((groups + 31) / 32);
+  const unsigned blocks = (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, kNumSMs * (nv > 2 ? 4 : 8));
+  if (nv <= 1) f.template operator()<1>(blocks);
+  else if (nv <= 2) f.template operator()<2>(blocks);
+  else if (nv <= 4) f.template operator()<4>(blocks);
+  else f.template operator()<kNV>(blocks);
 }
+struct XentShort {
+  const XentRows& d;
+  template <int NV>
+  void operator()(unsigned blocks) const { k_xent_rows_warp<NV><<<blocks, 32 * kWarps, 0, stream()>>>(d); }
+};
+struct DistillShort {
+  const Distill& d;
+  template <int NV>
+  void operator()(unsigned blocks) const { k_distill_rows_warp<NV><<<blocks, 32 * kWarps, 0, stream()>>>(d); }
+};
 
 }  // namespace
 
@@ -732,7 +773,7 @@ void xent_rows(const float* logits, float* planes, int64_t ld, int64_t n, int64_
   if (n == 0) return;
   const int pid = prof_begin_named("k_xent_rows", 8.0 * (double)n * (double)ld);
   const XentRows d{logits, planes, (int)ld, (int)V, n, targets, tgt_dtype, row0, nll, device_error_word()};
-  if (ld <= kShort) k_xent_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(d);
+  if (ld <= kShort) with_warp_rows(ld / 4, n, XentShort{d});
   else launch_ring(d, (int)(ld / 4));
   count_launch();
   after_launch("k_xent_rows");
@@ -794,10 +835,12 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   if (n) {
     const Distill d{x, ent, flag, count, n, V, (int)K, temperature, part, hd ? fptr(hd) : nullptr, parts,
                     device_error_word()};
-    k_teacher<<<grid_for((size_t)n * 32, 256), 256, (size_t)K * 32, stream()>>>(
+    if (K > 512)   // over 48 KB
+      MALUS_CUDA(cudaFuncSetAttribute(k_teacher, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K * 64));
+    k_teacher<<<grid_for((size_t)n * 32, 256), 256, (size_t)K * 64, stream()>>>(
         idp, idt, te, n, (int)K, V, kLog2e / temperature, ent, flag, count, device_error_word());
     const int pid = prof_begin_named("k_distill_rows", (hd ? 8.0 : 4.0) * (double)n * (double)V);
-    if (V <= kShort) k_distill_rows_warp<<<warp_row_blocks(n), 32 * kWarps, 0, stream()>>>(d);
+    if (V <= kShort) with_warp_rows(groups, n, DistillShort{d});
     else launch_ring(d, (int)groups);
     count_launch(2);
     after_launch("k_distill_rows");
