@@ -467,26 +467,97 @@ __device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, in
   return t >= 0 && t < limit;
 }
 
+// Rows of up to 1024 columns (C a multiple of 4, aligned), a warp each, held in
+// registers: their planes and, for the planes of the columns, the columns' largest
+// finite magnitudes over the kept rows (as bits, zeroed before), in the same pass.
+template <int NV>
+__global__ void __launch_bounds__(512, 1) k_split_rows_max(const float* __restrict__ src, int64_t R, int C, int Cp,
+                                                        __half* __restrict__ hi, __half* __restrict__ lo,
+                                                        float* __restrict__ inv, uint32_t* __restrict__ bits,
+                                                        const void* keep, int kdt, int64_t limit) {
+  extern __shared__ uint32_t sh[];   // [16][128 NV]
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  uint32_t cm[4 * NV] = {};
+  float4 next[NV];
+  bool next_in = false;
+  auto fetch = [&](int64_t r) {   // a row ahead
+    const float4* p = reinterpret_cast<const float4*>(src + r * C);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) next[k] = 4 * (k * 32 + lane) < C ? p[k * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    next_in = kept(keep, kdt, limit, r);
+  };
+  const int64_t step = (int64_t)gridDim.x * 16;
+  int64_t r = (int64_t)blockIdx.x * 16 + g;
+  if (r < R) fetch(r);
+  for (; r < R; r += step) {
+    float v[4 * NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      v[4 * k] = next[k].x; v[4 * k + 1] = next[k].y; v[4 * k + 2] = next[k].z; v[4 * k + 3] = next[k].w;
+    }
+    const bool in = next_in;
+    if (r + step < R) fetch(r + step);
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4 * NV; ++k) {
+      const uint32_t b = finite_bits(v[k]);
+      m = max(m, b);
+      cm[k] = max(cm[k], in ? b : 0u);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    float up, iv;
+    scale_for(m, &up, &iv);
+    if (lane == 0) inv[r] = iv;
+    __half *hr = hi + r * Cp, *lr = lo + r * Cp;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = 4 * (k * 32 + lane);
+      if (i < Cp) {
+        __align__(8) __half h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2(v[4 * k + j] * up, &h[j], &l[j]);
+        *reinterpret_cast<uint2*>(hr + i) = *reinterpret_cast<uint2*>(h);
+        *reinterpret_cast<uint2*>(lr + i) = *reinterpret_cast<uint2*>(l);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4 * NV; ++k) sh[g * 128 * NV + k * 32 + lane] = cm[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * NV; i += 512) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a = max(a, sh[k * 128 * NV + i]);
+    // slot i: lane i % 32, its element i / 32 (group i / 128, component i / 32 % 4)
+    const int c = 4 * (i / 128 * 32 + (i & 31)) + (i >> 5 & 3);
+    if (c < C && a) atomicMax(bits + c, a);
+  }
+}
+
 // bits[c] = largest finite magnitude of column c (as bits; zeroed before): 32 x W
-// columns per block, 32 warps on every 32nd row, a slice of rows per blockIdx.y
+// columns per block, 8 warps on every 8th row, a slice of rows per blockIdx.y
 template <int W>
-__global__ void __launch_bounds__(1024) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
-                                                  uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
-  __shared__ uint32_t sh[32][32 * W];
+__global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, int64_t R, int64_t C,
+                                                 uint32_t* __restrict__ bits, const void* keep, int kdt, int64_t limit) {
+  __shared__ uint32_t sh[8][32 * W];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * W;
   uint32_t m[W] = {};
   if (c < C) {
-    const int64_t step = (int64_t)gridDim.y * 32;
-    for (int64_t r = (int64_t)blockIdx.y * 32 + g; r < R; r += 8 * step) {
+    const int64_t step = (int64_t)gridDim.y * 8;
+    for (int64_t r = (int64_t)blockIdx.y * 8 + g; r < R; r += 8 * step) {
       float v[8][W];
       bool k[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t q = r + i * step < R ? r + i * step : r;   // past the end: the first one again
+      for (int i = 0; i < 8; ++i) {   // all in flight; past the end: the first one again
+        const int64_t q = r + i * step < R ? r + i * step : r;
         const float* p = src + q * C + c;
-        if constexpr (W == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(p);
-        else v[i][0] = *p;
+        if constexpr (W == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(p);
+          v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
+        } else {
+          v[i][0] = *p;
+        }
         k[i] = kept(keep, kdt, limit, q);
       }
 #pragma unroll
@@ -498,11 +569,12 @@ __global__ void __launch_bounds__(1024) k_col_max(const float* __restrict__ src,
 #pragma unroll
   for (int j = 0; j < W; ++j) sh[g][j * 32 + lane] = m[j];
   __syncthreads();
-  // warp g takes W of the columns: its lanes the 32 warps' maxima
-  for (int i = g; i < 32 * W; i += 32) {
-    const uint32_t a = __reduce_max_sync(0xffffffffu, sh[lane][i]);
-    const int64_t col = ((int64_t)blockIdx.x * 32 + (i & 31)) * W + (i >> 5);
-    if (lane == 0 && col < C) atomicMax(bits + col, a);   // a maximum: the order does not matter
+  if (threadIdx.x < 32 * W) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a = max(a, sh[k][threadIdx.x]);
+    const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * W + g;
+    if (col < C) atomicMax(bits + col, a);   // a maximum: the order does not matter
   }
 }
 
@@ -727,25 +799,84 @@ void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* 
   prof_end(pid);
 }
 
+namespace {
+
+void col_max(const float* src, int64_t R, int64_t C, uint32_t* bits, const void* keep, int keep_dtype, int64_t limit) {
+  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
+  const int64_t cb = vec ? (C + 127) / 128 : (C + 31) / 32;
+  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 63) / 64, kNumSMs * 4 / cb));   // one wave
+  if (vec) k_col_max<4><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  else k_col_max<1><<<dim3((unsigned)cb, ry), 256, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
+  count_launch();
+  after_launch("k_col_max");
+}
+
+void split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const uint32_t* bits,
+                const void* keep, int keep_dtype, int64_t limit) {
+  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
+  const int64_t Rp = pad64(R), step = (int64_t)65535 * 64;
+  for (int64_t r0 = 0; r0 < Rp; r0 += step) {   // grid.y holds 65535 tiles
+    const dim3 grid((unsigned)((C + 63) / 64), (unsigned)(std::min(step, Rp - r0) / 64));
+    const float* s = src + r0 * C;
+    const void* k = keep ? static_cast<const char*>(keep) + r0 * (int64_t)dtype_size(keep_dtype) : nullptr;
+    if (vec) k_split_cols<true><<<grid, 256, 0, stream()>>>(s, R - r0, C, Rp, bits, hi + r0, lo + r0, inv, k, keep_dtype, limit);
+    else k_split_cols<false><<<grid, 256, 0, stream()>>>(s, R - r0, C, Rp, bits, hi + r0, lo + r0, inv, k, keep_dtype, limit);
+    count_launch();
+  }
+  after_launch("k_split_cols");
+}
+
+uint32_t* zero_bits(int64_t C) {
+  uint32_t* bits = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
+  MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
+  return bits;
+}
+
+}  // namespace
+
 void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
                     int keep_dtype, int64_t limit) {
   if (C == 0) return;
-  const int64_t Rp = pad64(R);
-  uint32_t* bits = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
   const int pid = prof_begin(1, 0.0, 8.0 * (double)R * (double)C);
-  MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
-  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
-  const int64_t cb = vec ? (C + 127) / 128 : (C + 31) / 32;
-  // few slices: their maxima meet in one word per column
-  const unsigned ry = (unsigned)std::max<int64_t>(1, std::min<int64_t>((R + 255) / 256, (kNumSMs * 2 + cb - 1) / cb));
-  if (vec) k_col_max<4><<<dim3((unsigned)cb, ry), 1024, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
-  else k_col_max<1><<<dim3((unsigned)cb, ry), 1024, 0, stream()>>>(src, R, C, bits, keep, keep_dtype, limit);
-  if (Rp / 64 > 65535) panic("f16_split_cols of %lld rows", (long long)R);
-  const dim3 grid((unsigned)((C + 63) / 64), (unsigned)(Rp / 64));
-  if (vec) k_split_cols<true><<<grid, 256, 0, stream()>>>(src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
-  else k_split_cols<false><<<grid, 256, 0, stream()>>>(src, R, C, Rp, bits, hi, lo, inv, keep, keep_dtype, limit);
-  count_launch(2);
-  after_launch("k_split_cols");
+  uint32_t* bits = zero_bits(C);
+  col_max(src, R, C, bits, keep, keep_dtype, limit);
+  split_cols(src, R, C, hi, lo, inv, bits, keep, keep_dtype, limit);
+  scratch_free(bits);
+  prof_end(pid);
+}
+
+void f16_split_both(const float* src, int64_t R, int64_t C, __half* rhi, __half* rlo, float* rinv, __half* chi,
+                    __half* clo, float* cinv, const void* keep, int keep_dtype, int64_t limit) {
+  if (R == 0 || C == 0) return;
+  // one read for the rows' planes and the columns' maxima where a warp's registers
+  // hold a row: 16384 x 384 measured 11 us against 10 and 14 apart
+  if (C > 1024 || C % 4 || ((uintptr_t)src & 15)) {
+    f16_split_rows(src, R, C, rhi, rlo, rinv);
+    f16_split_cols(src, R, C, chi, clo, cinv, keep, keep_dtype, limit);
+    return;
+  }
+  const int pid = prof_begin(1, 0.0, 16.0 * (double)R * (double)C);
+  uint32_t* bits = zero_bits(C);
+  const int Cp = (int)pad64(C), nv = (Cp + 127) / 128;
+  const unsigned grid = (unsigned)std::min<int64_t>((R + 15) / 16, kNumSMs);   // few blocks: their maxima meet in one word per column
+  auto go = [&](auto kernel, int NV) {
+    const int smem = 16 * 128 * NV * 4;
+    MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<grid, 512, smem, stream()>>>(src, R, (int)C, Cp, rhi, rlo, rinv, bits, keep, keep_dtype, limit);
+  };
+  switch (nv) {
+    case 1: go(k_split_rows_max<1>, 1); break;
+    case 2: go(k_split_rows_max<2>, 2); break;
+    case 3: go(k_split_rows_max<3>, 3); break;
+    case 4: go(k_split_rows_max<4>, 4); break;
+    case 5: go(k_split_rows_max<5>, 5); break;
+    case 6: go(k_split_rows_max<6>, 6); break;
+    case 7: go(k_split_rows_max<7>, 7); break;
+    default: go(k_split_rows_max<8>, 8); break;
+  }
+  count_launch();
+  after_launch("k_split_rows_max");
+  split_cols(src, R, C, chi, clo, cinv, bits, keep, keep_dtype, limit);
   scratch_free(bits);
   prof_end(pid);
 }

@@ -48,6 +48,9 @@ void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target,
 void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv);
 void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
                     int keep_dtype, int64_t limit);
+// Both at once.
+void f16_split_both(const float* src, int64_t R, int64_t C, __half* rhi, __half* rlo, float* rinv, __half* chi,
+                    __half* clo, float* cinv, const void* keep, int keep_dtype, int64_t limit);
 inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // floats behind the scales of `rows` plane rows: a GEMM reads whole tiles of them

@@ -48,13 +48,16 @@ struct Planes {
 };
 
 void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
-           int64_t ld, const Planes& wv, const Planes& xr, const int* count, float* nll, float* dx, float* dw) {
-  // x by columns, tokens that are not counted as zeros: whatever they hold, dl
-  // is 0 there; weight by columns (tied) or rows: an embedding axis per row
-  Planes xc(dw ? D : 0, n), wd(dx ? D : 0, V);
-  if (dw) f16_split_cols(x, n, D, xc.hi, xc.lo, xc.inv, tgt, tdt, V);
-  if (dx && tied) f16_split_cols(w, V, D, wd.hi, wd.lo, wd.inv, nullptr, 0, 0);
-  if (dx && !tied) f16_split_rows(w, D, V, wd.hi, wd.lo, wd.inv);
+           int64_t ld, const int* count, float* nll, float* dx, float* dw) {
+  // a token, and a vocabulary entry, per row; then an embedding axis per row, with
+  // the tokens that are not counted as zeros: whatever they hold, dl is 0 there
+  Planes xr(n, D), wv(V, D), xc(dw ? D : 0, n), wd(dx ? D : 0, V);
+  if (dw) f16_split_both(x, n, D, xr.hi, xr.lo, xr.inv, xc.hi, xc.lo, xc.inv, tgt, tdt, V);
+  else f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
+  if (tied && dx) f16_split_both(w, V, D, wv.hi, wv.lo, wv.inv, wd.hi, wd.lo, wd.inv, nullptr, 0, 0);
+  else if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
+  else if (dx) f16_split_both(w, D, V, wd.hi, wd.lo, wd.inv, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
+  else f16_split_cols(w, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
   // pieces of whole 256-row tiles, of even size
   const bool in_place = xent_rows_in_place(ld);
   const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8))) / 256 * 256);
@@ -84,8 +87,12 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   scratch_free(logits);
 }
 
-void loss_only(const void* tgt, int tdt, int64_t n, int64_t D, int64_t V, const Planes& wv, const Planes& xr,
+void loss_only(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
                float* nll) {
+  Planes xr(n, D), wv(V, D);
+  f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
+  if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
+  else f16_split_cols(w, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
   const int parts = f16_lse_parts((int)V);
   const int64_t piece = std::min<int64_t>(n, kLossRows);
   float2* part = static_cast<float2*>(scratch_alloc((size_t)piece * (parts * 8 + 4)));
@@ -386,14 +393,10 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
     if (hw) MALUS_CUDA(cudaMemsetAsync(fptr(hw), 0, V * D * 4, stream()));
   } else {
     const int64_t N = (int64_t)n;
-    Planes wv(V, D);   // a vocabulary entry per row
-    if (tied) f16_split_rows(wp, V, D, wv.hi, wv.lo, wv.inv);
-    else f16_split_cols(wp, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
-    Planes xr(N, D);   // a token per row
-    f16_split_rows(xp, N, D, xr.hi, xr.lo, xr.inv);
-    if (hx || hw) train(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, ld, wv, xr, count, fptr(hn),
-                        hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
-    else loss_only(tp, tdt, N, (int64_t)D, (int64_t)V, wv, xr, fptr(hn));
+    if (hx || hw)
+      train(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, ld, count, fptr(hn), hx ? fptr(hx) : nullptr,
+            hw ? fptr(hw) : nullptr);
+    else loss_only(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, fptr(hn));
   }
   loss_mean(fptr(hn), (int64_t)n, count, fptr(loss));
   scratch_free(count);
