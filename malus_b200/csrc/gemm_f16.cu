@@ -45,7 +45,7 @@ constexpr int kRegsLaunch = 168, kRegsIo = 40, kRegsEpi = 232;
 static_assert(128 * kRegsIo + 32 * kEpiWarps * kRegsEpi <= kThreads * kRegsLaunch, "registers");
 constexpr int kStaging = 32 * 32 * 4;               // per epilogue warp: 32 rows x 32 columns
 constexpr int kSmem = STAGES * kStageBytes + 1024 + 256 + kEpiWarps * kStaging;
-static_assert(kSmem <= 232448, "shared memory");
+static_assert(kSmem <= 232448 && kCols == 128, "shared memory; a warp's lanes hold four column scales each");
 
 struct Params {
   int M, N, K, tiles_m, tiles_n, nst, splits;
@@ -97,16 +97,25 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t tile, bool mn) {
 
 enum Mode : int { kStore = 0, kLse = 1 };
 
-// The sums acc of 32 rows from m0 (one per lane), columns n0 .. n0 + kCols - 1:
+// v times the scales of four columns, which lane `from` holds.
+__device__ __forceinline__ float4 scale4(float4 v, float4 sb4, int from) {
+  v.x *= __shfl_sync(0xffffffffu, sb4.x, from);
+  v.y *= __shfl_sync(0xffffffffu, sb4.y, from);
+  v.z *= __shfl_sync(0xffffffffu, sb4.z, from);
+  v.w *= __shfl_sync(0xffffffffu, sb4.w, from);
+  return v;
+}
+
+// The sums acc of 32 rows from m0 (one per lane, scale sa), columns n0 .. n0 +
+// kCols - 1 (lane i holds the scales of columns 4 i .. 4 i + 3 of them):
 // scaled and sent to the output 32 columns at a time through the warp's staging
 // block, which a TMA store (or, accumulating, a TMA add: one per element and
 // launch, so the order is fixed) takes from there.  The copy drops what lies
 // past M or N.
 __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap* mOut, const Unit& un,
-                                             float (&acc)[kCols], int m0, int n0, float alpha, uint8_t* stage) {
-  const int lane = threadIdx.x & 31, m = m0 + lane;
+                                             float (&acc)[kCols], int m0, int n0, float sa, float4 sb4, uint8_t* stage) {
+  const int lane = threadIdx.x & 31;
   if (m0 >= p.M) return;   // uniform over the warp
-  const float sa = alpha * (p.a_inv && m < p.M ? p.a_inv[m] : 1.0f);
   float4* mine = reinterpret_cast<float4*>(stage + lane * 128);
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) {
@@ -117,10 +126,7 @@ __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap*
     for (int g = 0; g < 8; ++g) {   // 16-byte granule g of row r lies at g ^ (r & 7): the map's swizzle
       float4 v = make_float4(acc[c + 4 * g] * sa, acc[c + 4 * g + 1] * sa, acc[c + 4 * g + 2] * sa,
                              acc[c + 4 * g + 3] * sa);
-      if (p.b_inv) {   // padded to whole tiles by the host
-        const float4 sb = *reinterpret_cast<const float4*>(p.b_inv + n0 + c + 4 * g);
-        v.x *= sb.x; v.y *= sb.y; v.z *= sb.z; v.w *= sb.w;
-      }
+      v = scale4(v, sb4, c / 4 + g);
       mine[g ^ (lane & 7)] = v;
     }
     fence_async_smem();
@@ -134,15 +140,18 @@ __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap*
 }
 
 // The sums of a row into its maximum, sum of exponentials and target value.
-__device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols], int m, int n0, float alpha) {
-  if (m >= p.M) return;
-  const float sa = alpha * (p.a_inv ? p.a_inv[m] : 1.0f);
+__device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols], int m, int n0, float sa, float4 sb4) {
   float mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    acc[j] = n0 + j < p.N ? acc[j] * sa * p.b_inv[n0 + j] : -INFINITY;
-    mx = fmaxf(mx, acc[j]);
+  for (int j = 0; j < kCols; j += 4) {
+    const float4 v = scale4(make_float4(acc[j] * sa, acc[j + 1] * sa, acc[j + 2] * sa, acc[j + 3] * sa), sb4, j / 4);
+    acc[j] = n0 + j < p.N ? v.x : -INFINITY;
+    acc[j + 1] = n0 + j + 1 < p.N ? v.y : -INFINITY;
+    acc[j + 2] = n0 + j + 2 < p.N ? v.z : -INFINITY;
+    acc[j + 3] = n0 + j + 3 < p.N ? v.w : -INFINITY;
+    mx = fmaxf(mx, fmaxf(fmaxf(acc[j], acc[j + 1]), fmaxf(acc[j + 2], acc[j + 3])));
   }
+  if (m >= p.M) return;
   float s = 0.0f;
   const float mm = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
@@ -315,6 +324,11 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
     bool ok = true;
     for (int u = grp; u < total && ok; u += ngrp) {
       const Unit un = unit_at(p, u);
+      const int m0 = un.m0 + (int)rank * BM + quarter * 32, n0 = un.n0 + part * kCols;
+      // the scales, on their way while the sums come in (b's are padded to whole tiles)
+      const float sa = alpha * (p.a_inv && m0 + lane < p.M ? p.a_inv[m0 + lane] : 1.0f);
+      const float4 sb4 = p.b_inv ? *reinterpret_cast<const float4*>(p.b_inv + n0 + 4 * lane)
+                                 : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
       float acc[kCols];
       for (int st = un.st_lo; st < un.st_hi; st += kChunk, ++chunk) {
         const uint32_t b = chunk & 1;
@@ -340,9 +354,8 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
         if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acce[b]), 0));
       }
       if (!ok) break;
-      const int m0 = un.m0 + (int)rank * BM + quarter * 32, n0 = un.n0 + part * kCols;
-      if (MODE == kLse) finish_lse(p, acc, m0 + lane, n0, alpha);
-      else finish_store(p, &mOut, un, acc, m0, n0, alpha, stage);
+      if (MODE == kLse) finish_lse(p, acc, m0 + lane, n0, sa, sb4);
+      else finish_store(p, &mOut, un, acc, m0, n0, sa, sb4, stage);
       __syncwarp();   // rows past M return early: the next tensor memory load needs the whole warp
     }
     if (MODE == kStore && lane == 0) bulk_wait<0>();   // every copy is done before the CTA exits
