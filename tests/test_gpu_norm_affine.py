@@ -198,3 +198,18 @@ def test_through_the_tape(M, rt):
     for g, r, t, what in zip(got, ref[1:], tol[1:], ("dx", "dweight", "dbias")):
         within(g, r, t, what + " of the tape")
     rt.malus_tape_reset()
+
+
+@pytest.mark.parametrize("D,offs", [(100, (1, 1, 1)), (1101, (3, 3, 3)), (100, (1, 2, 1)), (66, (2, 2, 0)), (2050, (1, 1, 1))])
+def test_rows_off_the_16_byte_grid(M, rt, D, offs):
+    # x, dy and weight each so many floats past an aligned address; enough rows that a thread walks several
+    x, w, b, dy = inputs((3001, D), D)
+    ref, tol = reference(x, w, b, dy, 1e-5)
+    T = M.Tensor.from_numpy
+    keep = [T(np.concatenate([np.zeros(o, np.float32), a.ravel()])) for o, a in zip(offs, (x, dy, w))]
+    ox, od, ow = [M.Tensor.wrap(rt.malus_tensor_data(k.h) + 4 * o, s.shape) for k, o, s in zip(keep, offs, (x, dy, w))]
+    tb = T(b)
+    y, st = M.layernorm_affine(ox, ow, tb)
+    got = (y, *M.layernorm_affine_bwd(ox, ow, st, od))
+    for g, r, t, what in zip(got, ref, tol, ("y", "dx", "dweight", "dbias")):
+        within(g.numpy(), r, t, f"{what} D {D} offsets {offs}")
