@@ -180,6 +180,7 @@ SIGNATURES: dict[str, tuple] = {
     "malus_layernorm_affine_fwd": (i64, [i64, i64, i64, f32, P_i64]),
     "malus_layernorm_affine_bwd": (None, [i64, i64, i64, i64, P_i64, P_i64, P_i64]),
     "malus_linear_xent": (i64, [i64, i64, i64, i32, P_i64, P_i64, P_i64]),
+    "malus_linear_xent_mode": (i32, [i32]),
     "malus_distill": (i64, [i64, i64, i64, f32, P_i64, P_i64]),
     "tape_record_layernorm_affine": (None, [i64, i64, i64, i64, i64]),
     "tape_record_loss": (None, [P_i64, P_i64, sz, i64]),

@@ -19,6 +19,7 @@
 // are split twice, by rows and by columns, so that every product's operands are
 // scaled along the axis it does not sum over.
 #include "gemm_f16.cuh"
+#include "linear_xent.cuh"
 #include "loss_rows.cuh"
 
 namespace malus {
@@ -341,9 +342,11 @@ void few(const float* x, const float* w, const void* tgt, int tdt, bool tied, in
   scratch_free(part);
 }
 
+std::atomic<int> g_mode{-1};
+
 // Rows that take this path: x in shared memory beside the block's sums.
 bool few_rows(int64_t n, int64_t D) {
-  if (n < 1 || n > kFewRows) return false;
+  if (n < 1 || n > kFewRows || g_mode.load(std::memory_order_relaxed) != -1) return false;
   const int64_t N = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
   return N * (D + 127 + kFewWarps * 128) * 4 <= kFewSmem;
 }
@@ -354,6 +357,11 @@ bool few_rows(int64_t n, int64_t D) {
 using namespace malus;
 
 extern "C" {
+
+int32_t malus_linear_xent_mode(int32_t mode) {
+  if (mode < -1 || mode > 1) panic("malus_linear_xent_mode(%d): -1, 0 or 1", mode);
+  return g_mode.exchange(mode);
+}
 
 int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
                           int64_t* dweight) {
@@ -385,6 +393,16 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
     else tensor_release(hn);
     if (dx) *dx = 0;
     if (dweight) *dweight = 0;
+    return loss;
+  }
+  const int mode = g_mode.load(std::memory_order_relaxed);
+  if (n && (mode < 0 ? head_small((int64_t)n, (int64_t)D, (int64_t)V) : mode == 1 && n <= 16384)) {
+    head_small_run(xp, wp, tp, tdt, tied != 0, (int64_t)n, (int64_t)D, (int64_t)V, fptr(hn), fptr(loss),
+                   hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
+    if (nll) *nll = hn;
+    else tensor_release(hn);
+    if (dx) *dx = hx;
+    if (dweight) *dweight = hw;
     return loss;
   }
   int* count = static_cast<int*>(scratch_alloc(4));

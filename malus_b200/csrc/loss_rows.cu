@@ -136,31 +136,47 @@ __device__ __forceinline__ float4 less_hot(float4 q, int t, int e) {
   return q;
 }
 
+// PLANES: the gradient as half planes, else as f32 (in place).
+template <bool PLANES>
 struct XentRows {
   const float* logits;
-  float* out;          // the planes: over the logits, or memory of its own
+  float* out;          // the gradient: over the logits, or memory of its own (null: none)
   int ld, V_;
   int64_t rows;
   const void* tgt;
   int tdt;
   int64_t row0;
   float* nll;
+  int* count;          // counts the rows (null: someone else does)
   int32_t* err;
   __device__ __forceinline__ const float* row(int64_t r) const { return logits + r * ld; }
   __device__ __forceinline__ int width() const { return ld; }   // groups cover the pitch
   __device__ __forceinline__ int V() const { return V_; }       // logits among them
+  // four elements of a row's gradient
+  __device__ __forceinline__ void store(float* row_out, int e, float4 q) const {
+    if (PLANES) store_planes(row_out, ld, e, q);
+    else *reinterpret_cast<float4*>(row_out + e) = q;
+  }
+  // a row's value, by one thread
+  __device__ __forceinline__ void tell(int64_t r, int64_t t, bool counted, float v) const {
+    nll[row0 + r] = v;
+    if (!count) return;
+    if (counted) atomicAdd(count, 1);   // whole numbers: the order does not matter
+    else if (t >= V_) atomicExch(err, kErrId);
+  }
 };
 
-template <int NV>
-__global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d) {
+template <int NV, class Op>
+__global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const Op d) {
   const int lane = threadIdx.x & 31, ld = d.ld, V = d.V_;
   for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < d.rows; r += (int64_t)gridDim.x * kWarps) {
     const float* row = d.row(r);
     float* out = d.out + r * ld;
     const int64_t t = id_at(d.tgt, d.tdt, d.row0 + r);
     if (t < 0 || t >= V) {
-      if (lane == 0) d.nll[d.row0 + r] = 0.0f;
-      for (int g = lane; g < ld / 4; g += 32) store_planes(out, ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (lane == 0) d.tell(r, t, false, 0.0f);
+      if (!d.out) continue;
+      for (int g = lane; g < ld / 4; g += 32) d.store(out, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
       continue;
     }
     const float zt = row[t];
@@ -171,13 +187,14 @@ __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d
       v[k] = e + 4 <= V ? *reinterpret_cast<const float4*>(row + e) : load_edge(row, V, e);
     }
     const RowStat st = warp_stat(v, kLog2e);   // the whole row is in registers after it
-    if (lane == 0) d.nll[d.row0 + r] = logf(st.sum) - (zt - st.max);
+    if (lane == 0) d.tell(r, t, true, logf(st.sum) - (zt - st.max));
+    if (!d.out) continue;
     const float f = 1.0f / st.sum;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int e = 4 * (k * 32 + lane);
       if (e < ld)   // columns from V on hold exp(-inf) = 0
-        store_planes(out, ld, e, less_hot(make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f), (int)t, e));
+        d.store(out, e, less_hot(make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f), (int)t, e));
     }
   }
 }
@@ -587,8 +604,8 @@ __device__ __forceinline__ void ring_map(R_& R, RowStat st, float c, F&& f) {
   }
 }
 
-template <class R_>
-__device__ __forceinline__ void ring_rows(R_& R, const XentRows& d, float2* table, int64_t first, int64_t step) {
+template <class R_, bool PLANES>
+__device__ __forceinline__ void ring_rows(R_& R, const XentRows<PLANES>& d, float2* table, int64_t first, int64_t step) {
   const int tid = (int)threadIdx.x, nt = R.chunk / 2;
   int64_t next = first < d.rows ? id_at(d.tgt, d.tdt, d.row0 + first) : -1;
   uint32_t turn = 0;
@@ -598,18 +615,23 @@ __device__ __forceinline__ void ring_rows(R_& R, const XentRows& d, float2* tabl
     const int64_t t = next;
     if (r + step < d.rows) next = id_at(d.tgt, d.tdt, d.row0 + r + step);
     if (t < 0 || t >= d.V_) {
-      if (tid == 0) d.nll[d.row0 + r] = 0.0f;
+      if (tid == 0) d.tell(r, t, false, 0.0f);
       ring_skip(R, R_::STAY ? 1 : 2);   // the copies have left the row before it is written
       ring_barrier(R);
-      for (int g = tid; g < R.groups; g += nt) store_planes(out, d.ld, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (d.out)
+        for (int g = tid; g < R.groups; g += nt) d.store(out, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
       continue;
     }
     const float zt = tid == 0 ? row[t] : 0.0f;
-    const RowStat st = ring_stat(R, kLog2e, table, turn, false);   // its barrier: a row that stays has landed
-    if (tid == 0) d.nll[d.row0 + r] = logf(st.sum) - (zt - st.max);
+    const RowStat st = ring_stat(R, kLog2e, table, turn, !d.out);   // its barrier: a row that stays has landed
+    if (tid == 0) d.tell(r, t, true, logf(st.sum) - (zt - st.max));
+    if (!d.out) {
+      if (!R_::STAY) ring_skip(R, 1);
+      continue;
+    }
     const float f = 1.0f / st.sum;
     ring_map(R, st, kLog2e, [&](int g, float4 e) {   // columns from V on hold exp(-inf) = 0
-      store_planes(out, d.ld, 4 * g, less_hot(make_float4(e.x * f, e.y * f, e.z * f, e.w * f), (int)t, 4 * g));
+      d.store(out, 4 * g, less_hot(make_float4(e.x * f, e.y * f, e.z * f, e.w * f), (int)t, 4 * g));
     });
   }
 }
@@ -747,11 +769,22 @@ void with_warp_rows(int64_t groups, int64_t rows, F&& f) {
   else if (nv <= 4) f.template operator()<4>(blocks);
   else f.template operator()<kNV>(blocks);
 }
+template <bool PLANES>
 struct XentShort {
-  const XentRows& d;
+  const XentRows<PLANES>& d;
   template <int NV>
   void operator()(unsigned blocks) const { k_xent_rows_warp<NV><<<blocks, 32 * kWarps, 0, stream()>>>(d); }
 };
+template <bool PLANES>
+void run_xent(const XentRows<PLANES>& d) {
+  if (d.rows == 0) return;
+  const int pid = prof_begin_named("k_xent_rows", (d.out ? 8.0 : 4.0) * (double)d.rows * (double)d.ld);
+  if (d.ld <= kShort) with_warp_rows(d.ld / 4, d.rows, XentShort<PLANES>{d});
+  else launch_ring(d, d.ld / 4);
+  count_launch();
+  after_launch("k_xent_rows");
+  prof_end(pid);
+}
 struct DistillShort {
   const Distill& d;
   template <int NV>
@@ -770,14 +803,14 @@ bool xent_rows_in_place(int64_t ld) { return ld / 4 <= kRingGroups; }
 
 void xent_rows(const float* logits, float* planes, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype,
                int64_t row0, float* nll) {
-  if (n == 0) return;
-  const int pid = prof_begin_named("k_xent_rows", 8.0 * (double)n * (double)ld);
-  const XentRows d{logits, planes, (int)ld, (int)V, n, targets, tgt_dtype, row0, nll, device_error_word()};
-  if (ld <= kShort) with_warp_rows(ld / 4, n, XentShort{d});
-  else launch_ring(d, (int)(ld / 4));
-  count_launch();
-  after_launch("k_xent_rows");
-  prof_end(pid);
+  run_xent(XentRows<true>{logits, planes, (int)ld, (int)V, n, targets, tgt_dtype, row0, nll, nullptr,
+                          device_error_word()});
+}
+
+void xent_rows_f32(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, float* nll,
+                   int* count, bool grad) {
+  run_xent(XentRows<false>{logits, grad ? logits : nullptr, (int)ld, (int)V, n, targets, tgt_dtype, 0, nll, count,
+                           device_error_word()});
 }
 
 void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,

@@ -20,6 +20,12 @@ bool xent_rows_in_place(int64_t ld);
 void xent_rows(const float* logits, float* planes, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype,
                int64_t row0, float* nll);
 
+// The same with the gradient as f32 in place (none without grad), counting the rows
+// into count[0] (cleared before) and reporting targets at or past V.  A row takes
+// any length: f32 in place only ever overwrites what has been read.
+void xent_rows_f32(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, float* nll,
+                   int* count, bool grad);
+
 // nll[r] of n rows from the statistics of gemm_f16_lse
 void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,
                float* nll);
