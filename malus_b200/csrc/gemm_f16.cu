@@ -473,23 +473,42 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* _
   }
 }
 
-// Whether row r is kept; loaded beside the row, not before it.
-__device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, int64_t r) {
+// Whether row r is kept; loaded beside the row, not before it.  err: where to report
+// an id at or past the limit.
+__device__ __forceinline__ bool kept(const void* keep, int dt, int64_t limit, int64_t r, int32_t* err = nullptr) {
   if (!keep) return true;
   const int64_t t = dt == MALUS_I64 ? ((const int64_t*)keep)[r] : (int64_t)((const int32_t*)keep)[r];
+  if (err && t >= limit) atomicExch(err, 4);
   return t >= 0 && t < limit;
 }
+
+// Up to two matrices of C columns split in one launch: their blocks follow one another.
+struct SplitJobs {
+  F16Split j[2];
+  uint32_t* bits[2];
+  int blocks[2];
+  int* count;       // kept rows of the first (null: not wanted)
+  int32_t* err;
+};
 
 // Rows of up to 1024 columns (C a multiple of 4, aligned), a warp each, held in
 // registers: their planes and, for the planes of the columns, the columns' largest
 // finite magnitudes over the kept rows (as bits, zeroed before), in the same pass.
 template <int NV>
-__global__ void __launch_bounds__(512, 1) k_split_rows_max(const float* __restrict__ src, int64_t R, int C, int Cp,
-                                                        __half* __restrict__ hi, __half* __restrict__ lo,
-                                                        float* __restrict__ inv, uint32_t* __restrict__ bits,
-                                                        const void* keep, int kdt, int64_t limit) {
+__global__ void __launch_bounds__(512, 1) k_split_rows_max(const SplitJobs jobs, int C, int Cp) {
   extern __shared__ uint32_t sh[];   // [16][128 NV]
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int which = (int)blockIdx.x >= jobs.blocks[0], block = (int)blockIdx.x - (which ? jobs.blocks[0] : 0);
+  const F16Split& job = jobs.j[which];
+  const float* __restrict__ src = job.src;
+  const int64_t R = job.R, limit = job.limit;
+  __half* __restrict__ hi = job.rhi;
+  __half* __restrict__ lo = job.rlo;
+  float* __restrict__ inv = job.rinv;
+  uint32_t* __restrict__ bits = jobs.bits[which];
+  const void* keep = job.keep;
+  const int kdt = job.keep_dtype;
+  int rows_kept = 0;
   uint32_t cm[4 * NV] = {};
   float4 next[NV];
   bool next_in = false;
@@ -497,12 +516,13 @@ __global__ void __launch_bounds__(512, 1) k_split_rows_max(const float* __restri
     const float4* p = reinterpret_cast<const float4*>(src + r * C);
 #pragma unroll
     for (int k = 0; k < NV; ++k) next[k] = 4 * (k * 32 + lane) < C ? p[k * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-    next_in = kept(keep, kdt, limit, r);
+    next_in = kept(keep, kdt, limit, r, lane == 0 ? jobs.err : nullptr);
   };
-  const int64_t step = (int64_t)gridDim.x * 16;
-  int64_t r = (int64_t)blockIdx.x * 16 + g;
+  const int64_t step = (int64_t)jobs.blocks[which] * 16;
+  int64_t r = (int64_t)block * 16 + g;
   if (r < R) fetch(r);
   for (; r < R; r += step) {
+    rows_kept += next_in;
     float v[4 * NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -545,6 +565,7 @@ __global__ void __launch_bounds__(512, 1) k_split_rows_max(const float* __restri
     const int c = 4 * (i / 128 * 32 + (i & 31)) + (i >> 5 & 3);
     if (c < C && a) atomicMax(bits + c, a);
   }
+  if (which == 0 && jobs.count && lane == 0 && rows_kept) atomicAdd(jobs.count, rows_kept);
 }
 
 // bits[c] = largest finite magnitude of column c (as bits; zeroed before): 32 x W
@@ -594,15 +615,21 @@ __global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, 
 // 64 x 64 tiles through shared memory: rows of the source in (16-byte groups when
 // VEC), columns out, 4 rows (8 bytes of a plane) per lane.
 template <bool VEC>
-__global__ void __launch_bounds__(256) k_split_cols(const float* __restrict__ src, int64_t R, int64_t C, int64_t Rp,
-                                                    const uint32_t* __restrict__ bits, __half* __restrict__ hi,
-                                                    __half* __restrict__ lo, float* __restrict__ inv, const void* keep,
-                                                    int kdt, int64_t limit) {
+__global__ void __launch_bounds__(256) k_split_cols(const SplitJobs jobs, int64_t C) {
   __shared__ float tile[64][65];
   __shared__ float ups[64];
   __shared__ uint32_t rows_kept[2];
-  const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * 64;
-  const int nr = (int)min((int64_t)64, R - r0), nc = (int)min((int64_t)64, C - c0), t = threadIdx.x;   // nr may be < 0
+  // blocks[i] tiles of 64 rows each, 64-column tiles side by side
+  const int ct = (int)((C + 63) / 64);
+  const int64_t c0 = (int64_t)(blockIdx.x % ct) * 64;
+  int rt = (int)(blockIdx.x / ct);
+  const int which = rt >= jobs.blocks[0];
+  if (which) rt -= jobs.blocks[0];
+  const F16Split& job = jobs.j[which];
+  const float* __restrict__ src = job.src;
+  const uint32_t* __restrict__ bits = jobs.bits[which];
+  const int64_t R = job.R, Rp = pad64(R), r0 = (int64_t)rt * 64;
+  const int nr = (int)min((int64_t)64, R - r0), nc = (int)min((int64_t)64, C - c0), t = threadIdx.x;
   const float* p = src + r0 * C + c0;
   constexpr int kStep = VEC ? 16 : 4;                     // rows between a thread's
   const int tx = VEC ? (t & 15) * 4 : t & 63, ty = VEC ? t >> 4 : t >> 6;
@@ -620,21 +647,21 @@ __global__ void __launch_bounds__(256) k_split_cols(const float* __restrict__ sr
     for (int i = 0; i < 16; ++i, q += 4 * C) v[i] = ty + 4 * i < nr && tx < nc ? *q : 0.0f;
   }
   if (t < 64) {
-    const bool k = t < nr && kept(keep, kdt, limit, r0 + t);
+    const bool k = t < nr && kept(job.keep, job.keep_dtype, job.limit, r0 + t);
     const uint32_t b = __ballot_sync(0xffffffffu, k);
     if ((t & 31) == 0) rows_kept[t >> 5] = b;
     float up = 1.0f, iv = 1.0f;
     if (t < nc) scale_for(bits[c0 + t], &up, &iv);
     ups[t] = up;
-    if (blockIdx.y == 0 && t < nc) inv[c0 + t] = iv;
+    if (rt == 0 && t < nc) job.cinv[c0 + t] = iv;
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) tile[ty + kStep * (VEC ? i >> 2 : i)][tx + (VEC ? i & 3 : 0)] = v[i];
   __syncthreads();
   const int r = (t & 15) * 4;
   const uint32_t k4 = rows_kept[r >> 5] >> (r & 31);
-  __half* h0 = hi + c0 * Rp + r0 + r;
-  __half* l0 = lo + c0 * Rp + r0 + r;
+  __half* h0 = job.chi + c0 * Rp + r0 + r;
+  __half* l0 = job.clo + c0 * Rp + r0 + r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = (t >> 4) + 16 * i;
@@ -824,58 +851,71 @@ void col_max(const float* src, int64_t R, int64_t C, uint32_t* bits, const void*
   after_launch("k_col_max");
 }
 
-void split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const uint32_t* bits,
-                const void* keep, int keep_dtype, int64_t limit) {
-  const bool vec = C % 4 == 0 && ((uintptr_t)src & 15) == 0;
-  const int64_t Rp = pad64(R), step = (int64_t)65535 * 64;
-  for (int64_t r0 = 0; r0 < Rp; r0 += step) {   // grid.y holds 65535 tiles
-    const dim3 grid((unsigned)((C + 63) / 64), (unsigned)(std::min(step, Rp - r0) / 64));
-    const float* s = src + r0 * C;
-    const void* k = keep ? static_cast<const char*>(keep) + r0 * (int64_t)dtype_size(keep_dtype) : nullptr;
-    if (vec) k_split_cols<true><<<grid, 256, 0, stream()>>>(s, R - r0, C, Rp, bits, hi + r0, lo + r0, inv, k, keep_dtype, limit);
-    else k_split_cols<false><<<grid, 256, 0, stream()>>>(s, R - r0, C, Rp, bits, hi + r0, lo + r0, inv, k, keep_dtype, limit);
-    count_launch();
+void split_cols(SplitJobs jobs, int n, int64_t C, bool vec) {
+  int64_t tiles = 0;
+  for (int i = 0; i < 2; ++i) {
+    jobs.blocks[i] = i < n ? (int)(pad64(jobs.j[i].R) / 64) : 0;
+    tiles += jobs.blocks[i];
   }
+  const int64_t blocks = tiles * ((C + 63) / 64);
+  if (blocks > INT32_MAX) panic("f16_split: %lld tiles", (long long)blocks);
+  if (vec) k_split_cols<true><<<(unsigned)blocks, 256, 0, stream()>>>(jobs, C);
+  else k_split_cols<false><<<(unsigned)blocks, 256, 0, stream()>>>(jobs, C);
+  count_launch();
   after_launch("k_split_cols");
-}
-
-uint32_t* zero_bits(int64_t C) {
-  uint32_t* bits = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
-  MALUS_CUDA(cudaMemsetAsync(bits, 0, (size_t)C * 4, stream()));
-  return bits;
 }
 
 }  // namespace
 
-void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
-                    int keep_dtype, int64_t limit) {
-  if (C == 0) return;
-  const int pid = prof_begin(1, 0.0, 8.0 * (double)R * (double)C);
-  uint32_t* bits = zero_bits(C);
-  col_max(src, R, C, bits, keep, keep_dtype, limit);
-  split_cols(src, R, C, hi, lo, inv, bits, keep, keep_dtype, limit);
-  scratch_free(bits);
+void f16_split_cols(const F16Split& job, int64_t C) {
+  if (C == 0 || job.R == 0) return;
+  const int pid = prof_begin(1, 0.0, 8.0 * (double)job.R * (double)C);
+  SplitJobs jobs{};
+  jobs.j[0] = job;
+  jobs.bits[0] = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
+  MALUS_CUDA(cudaMemsetAsync(jobs.bits[0], 0, (size_t)C * 4, stream()));
+  col_max(job.src, job.R, C, jobs.bits[0], job.keep, job.keep_dtype, job.limit);
+  split_cols(jobs, 1, C, C % 4 == 0 && ((uintptr_t)job.src & 15) == 0);
+  scratch_free(jobs.bits[0]);
   prof_end(pid);
 }
 
-void f16_split_both(const float* src, int64_t R, int64_t C, __half* rhi, __half* rlo, float* rinv, __half* chi,
-                    __half* clo, float* cinv, const void* keep, int keep_dtype, int64_t limit) {
-  if (R == 0 || C == 0) return;
+bool f16_split_both(const F16Split* job, int n, int64_t C, uint32_t* bits, int* count) {
   // one read for the rows' planes and the columns' maxima where a warp's registers
-  // hold a row: 16384 x 384 measured 11 us against 10 and 14 apart
-  if (C > 1024 || C % 4 || ((uintptr_t)src & 15)) {
-    f16_split_rows(src, R, C, rhi, rlo, rinv);
-    f16_split_cols(src, R, C, chi, clo, cinv, keep, keep_dtype, limit);
-    return;
+  // hold a row: 50304 x 768 measured 47 us (the copy rate) against 52 and 33 apart
+  bool fit = C <= 1024 && C % 4 == 0;
+  double bytes = 0.0;
+  for (int i = 0; i < n; ++i) {
+    fit = fit && ((uintptr_t)job[i].src & 15) == 0;
+    bytes += 16.0 * (double)job[i].R * (double)C;
   }
-  const int pid = prof_begin(1, 0.0, 16.0 * (double)R * (double)C);
-  uint32_t* bits = zero_bits(C);
+  if (!fit) {
+    for (int i = 0; i < n; ++i) {
+      f16_split_rows(job[i].src, job[i].R, C, job[i].rhi, job[i].rlo, job[i].rinv);
+      f16_split_cols(job[i], C);
+    }
+    return false;
+  }
+  const int pid = prof_begin(1, 0.0, bytes);
+  SplitJobs jobs{};
+  jobs.count = count;
+  jobs.err = device_error_word();
+  // one block per SM over both, by their rows: the maxima meet in one word per column
+  double rows = 0.0;
+  for (int i = 0; i < n; ++i) rows += (double)job[i].R;
+  unsigned grid = 0;
+  for (int i = 0; i < n; ++i) {
+    jobs.j[i] = job[i];
+    jobs.bits[i] = bits + i * C;
+    const int64_t most = std::max<int64_t>(1, (int64_t)(kNumSMs * ((double)job[i].R / rows)));
+    jobs.blocks[i] = (int)std::min<int64_t>((job[i].R + 15) / 16, most);
+    grid += (unsigned)jobs.blocks[i];
+  }
   const int Cp = (int)pad64(C), nv = (Cp + 127) / 128;
-  const unsigned grid = (unsigned)std::min<int64_t>((R + 15) / 16, kNumSMs);   // few blocks: their maxima meet in one word per column
   auto go = [&](auto kernel, int NV) {
     const int smem = 16 * 128 * NV * 4;
     MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<grid, 512, smem, stream()>>>(src, R, (int)C, Cp, rhi, rlo, rinv, bits, keep, keep_dtype, limit);
+    kernel<<<grid, 512, smem, stream()>>>(jobs, (int)C, Cp);
   };
   switch (nv) {
     case 1: go(k_split_rows_max<1>, 1); break;
@@ -889,9 +929,9 @@ void f16_split_both(const float* src, int64_t R, int64_t C, __half* rhi, __half*
   }
   count_launch();
   after_launch("k_split_rows_max");
-  split_cols(src, R, C, chi, clo, cinv, bits, keep, keep_dtype, limit);
-  scratch_free(bits);
+  split_cols(jobs, n, C, true);
   prof_end(pid);
+  return true;
 }
 
 }  // namespace malus

@@ -40,18 +40,29 @@ void gemm_f16(const F16Gemm& g);
 int f16_lse_parts(int N);
 void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target, int tgt_dtype);
 
-// Planes of a row-major R x C matrix: its rows (hi/lo [R][pad64(C)], inv[R]), or
-// its columns (hi/lo [C][pad64(R)], inv[C]).  Each plane row is scaled by the
+// Planes of a row-major R x C matrix: its rows (rhi/rlo [R][pad64(C)], rinv[R]), and
+// its columns (chi/clo [C][pad64(R)], cinv[C]).  Each plane row is scaled by the
 // power of two that brings its largest finite magnitude into [2^13, 2^14).
 // keep (columns only, may be null): rows whose keep id lies outside [0, limit)
 // are taken as zeros.
+struct F16Split {
+  const float* src;
+  int64_t R;
+  __half *rhi, *rlo;
+  float* rinv;
+  __half *chi, *clo;
+  float* cinv;
+  const void* keep;
+  int keep_dtype;
+  int64_t limit;
+};
 void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv);
-void f16_split_cols(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv, const void* keep,
-                    int keep_dtype, int64_t limit);
-// Both at once.
-void f16_split_both(const float* src, int64_t R, int64_t C, __half* rhi, __half* rlo, float* rinv, __half* chi,
-                    __half* clo, float* cinv, const void* keep, int keep_dtype, int64_t limit);
-inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+void f16_split_cols(const F16Split& job, int64_t C);
+// Both of one or two matrices (R > 0) of C columns.  bits: n * C words, zero.
+// Returns whether count[0] (zero before) now has the first one's kept rows, and ids
+// at or past its limit are reported in the error word.
+bool f16_split_both(const F16Split* jobs, int n, int64_t C, uint32_t* bits, int* count);
+__host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // floats behind the scales of `rows` plane rows: a GEMM reads whole tiles of them
 inline int64_t f16_scales(int64_t rows) { return (rows + 255) / 256 * 256; }

@@ -17,8 +17,10 @@ namespace cg = cooperative_groups;
 namespace malus {
 namespace {
 
-constexpr int kCluster = 8, kThreads = 256, BK = 16;
-constexpr int kTileFloats = 64 * 64;
+constexpr int kCluster = 8, kThreads = 256, BK = 32;
+// one stage of both operands, [BK][rows + 4] each, for either tile shape
+constexpr int kStage = BK * (16 + 4 + 128 + 4);
+static_assert(kStage >= BK * (64 + 4 + 64 + 4) && 2 * kStage >= 64 * 64 && 8 * kStage <= 48 * 1024, "shared memory");
 
 // out[m * ldo + n] = sum_k a(m, k) b(n, k), element (i, k) at i * s + k * sk; divided
 // by max(1, count[0]) where count is set.
@@ -31,73 +33,94 @@ struct Mul {
   int tiles_n, tiles;
   int narrow;      // 16 x 128 tiles, else 64 x 64
   int split;       // a cluster per tile
-  int keep_a, keep_b;   // k is a token: that operand's tokens that are not counted read as zeros
+  // That operand is x along the tokens, against dl: what is not finite reads as 0.
+  // A token that is not counted has dl = 0, whatever its x holds; in one that is,
+  // an x that is not finite has made its whole row of dl NaN already.
+  int finite_a, finite_b;
 };
 struct Small {
   Mul m[2];
   int blocks[2];   // of each product, multiples of kCluster
   int* count;
   int clear, use_count;
-  const void* tgt;
-  int tdt;
-  int64_t V;
   float *nll, *loss;   // with loss: one more cluster, whose first block takes the mean
   int64_t n;
 };
 
-__device__ __forceinline__ bool counted(const Small& s, int k) {
-  const int64_t t = s.tdt == MALUS_I64 ? ((const int64_t*)s.tgt)[k] : (int64_t)((const int32_t*)s.tgt)[k];
-  return t >= 0 && t < s.V;
-}
+// This thread's elements of an operand's [ROWS][BK] blocks along K.  Where K is
+// contiguous a warp takes 8 of K (32 bytes) of 4 rows, which falls into 32 different
+// banks, and the thread's elements are 8 rows apart; else a warp takes 32 rows (16
+// of them twice), and the thread's elements lie along K.
+template <int ROWS>
+struct Walk {
+  static constexpr int kPer = ROWS * BK / kThreads, kPitch = ROWS + 4;
+  const float* p;
+  int64_t step, advance;   // to the thread's next element; to the next block
+  int i, k, di, dk, n;
+  int at, at_step;         // in shared memory
+  bool finite;
 
-// This thread's elements of an operand's [ROWS][BK] block into v.
-template <int ROWS>
-__device__ __forceinline__ void fetch(const Small& s, const float* __restrict__ p, int64_t si, int64_t sk, int i0, int n,
-                                      int k0, int k1, bool keep, float (&v)[ROWS * BK / kThreads]) {
-#pragma unroll
-  for (int j = 0; j < ROWS * BK / kThreads; ++j) {
-    const int e = threadIdx.x + j * kThreads;
-    // lanes along whichever index is contiguous
-    const int i = i0 + (sk == 1 ? e / BK : e % ROWS), k = k0 + (sk == 1 ? e % BK : e / ROWS);
-    v[j] = i < n && k < k1 && (!keep || counted(s, k)) ? p[i * si + k * sk] : 0.0f;
+  __device__ __forceinline__ Walk(const float* base, int64_t si, int64_t sk, int i0, int rows, int k0, bool finite_only) {
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const bool kc = sk == 1;
+    i = kc ? w / 4 * 4 + lane / 8 : t % ROWS;
+    k = kc ? w % 4 * 8 + lane % 8 : t / ROWS;
+    di = kc ? 8 : 0;
+    dk = kc ? 0 : kThreads / ROWS;
+    at = k * kPitch + i;
+    at_step = kc ? 8 : dk * kPitch;
+    i += i0;
+    k += k0;
+    n = rows;
+    p = base + i * si + k * sk;
+    step = kc ? 8 * si : dk * sk;
+    advance = BK * sk;
+    finite = finite_only;
   }
-}
-template <int ROWS>
-__device__ __forceinline__ void put(float* sh, int64_t sk, const float (&v)[ROWS * BK / kThreads]) {
+  __device__ __forceinline__ void fetch(int k1, float (&v)[kPer]) {
 #pragma unroll
-  for (int j = 0; j < ROWS * BK / kThreads; ++j) {
-    const int e = threadIdx.x + j * kThreads;
-    const int i = sk == 1 ? e / BK : e % ROWS, k = sk == 1 ? e % BK : e / ROWS;
-    sh[k * (ROWS + 4) + i] = v[j];
+    for (int j = 0; j < kPer; ++j) {
+      v[j] = i + j * di < n && k + j * dk < k1 ? p[j * step] : 0.0f;
+      if (finite && !isfinite(v[j])) v[j] = 0.0f;
+    }
+    p += advance;
+    k += BK;
   }
-}
+  __device__ __forceinline__ void put(float* sh, const float (&v)[kPer]) const {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sh[at + j * at_step] = v[j];
+  }
+};
 
 // Tile `tile` of product m over K slice [k0, k1): TM x 4 sums per thread, left in
-// sum[BM][BN] of shared memory.
+// sh as [BM][BN].  Two stages: while one is multiplied the next one's loads run.
 template <int BM, int BN, int TM>
-__device__ __forceinline__ void tile_sums(const Small& s, const Mul& m, int tile, int k0, int k1, float* sh, float* sum) {
-  static_assert(BM * BN == kThreads * TM * 4, "tile");
-  float* as = sh;
-  float* bs = sh + BK * (BM + 4);
+__device__ __forceinline__ void tile_sums(const Mul& m, int tile, int k0, int k1, float* sh) {
+  static_assert(BM * BN == kThreads * TM * 4 && BK * (BM + 4 + BN + 4) <= kStage, "tile");
   const int m0 = tile / m.tiles_n * BM, n0 = tile % m.tiles_n * BN;
   const int tx = threadIdx.x % (BN / 4), ty = threadIdx.x / (BN / 4);
   float acc[TM][4] = {};
-  float va[BM * BK / kThreads], vb[BN * BK / kThreads];
-  fetch<BM>(s, m.a, m.sam, m.sak, m0, m.M, k0, k1, m.keep_a, va);
-  fetch<BN>(s, m.b, m.sbn, m.sbk, n0, m.N, k0, k1, m.keep_b, vb);
-  for (int k = k0; k < k1; k += BK) {
-    put<BM>(as, m.sak, va);
-    put<BN>(bs, m.sbk, vb);
-    __syncthreads();
-    if (k + BK < k1) {   // the next block's loads run under this one's arithmetic
-      fetch<BM>(s, m.a, m.sam, m.sak, m0, m.M, k + BK, k1, m.keep_a, va);
-      fetch<BN>(s, m.b, m.sbn, m.sbk, n0, m.N, k + BK, k1, m.keep_b, vb);
+  Walk<BM> wa(m.a, m.sam, m.sak, m0, m.M, k0, m.finite_a);
+  Walk<BN> wb(m.b, m.sbn, m.sbk, n0, m.N, k0, m.finite_b);
+  float va[Walk<BM>::kPer], vb[Walk<BN>::kPer];
+  wa.fetch(k1, va);
+  wb.fetch(k1, vb);
+  int stage = 0;
+  for (int k = k0; k < k1; k += BK, stage ^= 1) {
+    float* as = sh + stage * kStage;
+    float* bs = as + BK * (BM + 4);
+    wa.put(as, va);
+    wb.put(bs, vb);
+    __syncthreads();   // also: everyone is done with this stage's last block but one
+    if (k + BK < k1) {
+      wa.fetch(k1, va);
+      wb.fetch(k1, vb);
     }
 #pragma unroll
     for (int q = 0; q < BK; ++q) {
       float a[TM];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = as[q * (BM + 4) + ty * TM + i];
+      if constexpr (TM == 4) *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(as + q * (BM + 4) + ty * 4);
+      else *reinterpret_cast<float2*>(a) = *reinterpret_cast<const float2*>(as + q * (BM + 4) + ty * 2);
       const float4 b = *reinterpret_cast<const float4*>(bs + q * (BN + 4) + tx * 4);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
@@ -107,11 +130,11 @@ __device__ __forceinline__ void tile_sums(const Small& s, const Mul& m, int tile
         acc[i][3] = fmaf(a[i], b.w, acc[i][3]);
       }
     }
-    __syncthreads();
   }
+  __syncthreads();   // the operands make room for the sums
 #pragma unroll
   for (int i = 0; i < TM; ++i)
-    *reinterpret_cast<float4*>(sum + (ty * TM + i) * BN + tx * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    *reinterpret_cast<float4*>(sh + (ty * TM + i) * BN + tx * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
 }
 
 // Elements [first, last) of the tile: the sum of the `parts` blocks' tiles, out.
@@ -133,8 +156,7 @@ __device__ __forceinline__ void tile_out(const Mul& m, int tile, cg::cluster_gro
 }
 
 __global__ void __launch_bounds__(kThreads) k_head_small(const Small s) {
-  __shared__ __align__(16) float sh[BK * (64 + 4 + 64 + 4) + BK * 16];   // both tile shapes' operands
-  __shared__ __align__(16) float sum[kTileFloats];
+  __shared__ __align__(16) float sh[2 * kStage];
   __shared__ double red[kThreads / 32];
   cg::cluster_group cl = cg::this_cluster();
   int b = (int)blockIdx.x;
@@ -162,19 +184,19 @@ __global__ void __launch_bounds__(kThreads) k_head_small(const Small s) {
   const int k0 = m.split ? (int)((int64_t)m.K * rank / kCluster) : 0;
   const int k1 = m.split ? (int)((int64_t)m.K * (rank + 1) / kCluster) : m.K;
   const float f = s.use_count ? 1.0f / (float)max(1, *s.count) : 1.0f;
-  if (m.narrow) tile_sums<16, 128, 2>(s, m, tile, k0, k1, sh, sum);
-  else tile_sums<64, 64, 4>(s, m, tile, k0, k1, sh, sum);
+  if (m.narrow) tile_sums<16, 128, 2>(m, tile, k0, k1, sh);
+  else tile_sums<64, 64, 4>(m, tile, k0, k1, sh);
   const int size = m.narrow ? 16 * 128 : 64 * 64;
   if (!m.split) {
     __syncthreads();
-    if (m.narrow) tile_out<16, 128>(m, tile, cl, sum, 1, 0, size, f);
-    else tile_out<64, 64>(m, tile, cl, sum, 1, 0, size, f);
+    if (m.narrow) tile_out<16, 128>(m, tile, cl, sh, 1, 0, size, f);
+    else tile_out<64, 64>(m, tile, cl, sh, 1, 0, size, f);
     return;
   }
   cl.sync();
   const int first = size / kCluster * rank, last = first + size / kCluster;
-  if (m.narrow) tile_out<16, 128>(m, tile, cl, sum, kCluster, first, last, f);
-  else tile_out<64, 64>(m, tile, cl, sum, kCluster, first, last, f);
+  if (m.narrow) tile_out<16, 128>(m, tile, cl, sh, kCluster, first, last, f);
+  else tile_out<64, 64>(m, tile, cl, sh, kCluster, first, last, f);
   cl.sync();   // the others may still read this block's tile
 }
 
@@ -186,7 +208,7 @@ int plan(Mul& m) {
   const int bm = m.narrow ? 16 : 64, bn = m.narrow ? 128 : 64;
   m.tiles_n = (m.N + bn - 1) / bn;
   m.tiles = (m.M + bm - 1) / bm * m.tiles_n;
-  m.split = m.tiles < kNumSMs && m.K >= kCluster * 2 * BK;
+  m.split = m.tiles < kNumSMs && m.K >= kCluster * BK;
   return m.split ? m.tiles * kCluster : (m.tiles + kCluster - 1) / kCluster * kCluster;
 }
 
@@ -209,10 +231,17 @@ void launch(const Small& s) {
 
 }  // namespace
 
-bool head_small(int64_t n, int64_t D, int64_t V) {
-  // multiply-adds of a product, rows of x padded to the tile
-  const double rows = n <= 16 ? 16.0 : (double)((n + 63) / 64 * 64);
-  return n <= 16384 && rows * (double)D * (double)V <= kHeadSmallWork;
+// Measured against half planes, the whole call: training 128 x 181 x 1586 45 us
+// against 99, 256 x 384 x 1000 (9.8e7) 60 against 72, 256 x 768 x 1000 (2.0e8) 84
+// against 75; and 100 x 100 x 10000 (1.3e8) 119 against 78, 16384 x 64 x 64 (6.7e7)
+// 147 against 79, where a gradient sums over more than its slices can hide.  The
+// loss alone sums over D only: 64 x 384 x 2000 (4.9e7) 23 against 33, 256 x 384 x
+// 1000 (9.8e7) 31 against 32, 1000 x 384 x 500 (2.0e8) 46 against 32.
+bool head_small(int64_t n, int64_t D, int64_t V, bool grad) {
+  const double rows = n <= 16 ? 16.0 : (double)((n + 63) / 64 * 64);   // of x, padded to the tile
+  const double work = rows * (double)D * (double)V;
+  if (n > 16384) return false;
+  return grad ? work <= 1.0e8 && std::max(n, V) <= 2560 : work <= 6.0e7;
 }
 
 void head_small_run(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
@@ -222,9 +251,6 @@ void head_small_run(const float* x, const float* w, const void* tgt, int tdt, bo
   int* count = reinterpret_cast<int*>(logits + n * ld);
   Small s{};
   s.count = count;
-  s.tgt = tgt;
-  s.tdt = tdt;
-  s.V = V;
   s.n = n;
   s.clear = 1;
   const int N = (int)n, Di = (int)D, Vi = (int)V;
@@ -251,10 +277,10 @@ void head_small_run(const float* x, const float* w, const void* tgt, int tdt, bo
     if (dw) {
       if (tied) {
         g.m[i] = Mul{logits, x, 1, ld, 1, D, Vi, Di, N, dw, D};
-        g.m[i].keep_b = 1;
+        g.m[i].finite_b = 1;
       } else {
         g.m[i] = Mul{x, logits, 1, D, 1, ld, Di, Vi, N, dw, V};
-        g.m[i].keep_a = 1;
+        g.m[i].finite_a = 1;
       }
       g.blocks[i] = plan(g.m[i]);
     }

@@ -49,16 +49,30 @@ struct Planes {
 };
 
 void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
-           int64_t ld, const int* count, float* nll, float* dx, float* dw) {
+           int64_t ld, float* nll, float* loss, float* dx, float* dw) {
   // a token, and a vocabulary entry, per row; then an embedding axis per row, with
   // the tokens that are not counted as zeros: whatever they hold, dl is 0 there
   Planes xr(n, D), wv(V, D), xc(dw ? D : 0, n), wd(dx ? D : 0, V);
-  if (dw) f16_split_both(x, n, D, xr.hi, xr.lo, xr.inv, xc.hi, xc.lo, xc.inv, tgt, tdt, V);
-  else f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
-  if (tied && dx) f16_split_both(w, V, D, wv.hi, wv.lo, wv.inv, wd.hi, wd.lo, wd.inv, nullptr, 0, 0);
-  else if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
-  else if (dx) f16_split_both(w, D, V, wd.hi, wd.lo, wd.inv, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
-  else f16_split_cols(w, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
+  // the row count, and the column maxima of x and of weight
+  const size_t words = 4 + (size_t)(D + std::max(D, V));
+  int* count = static_cast<int*>(scratch_alloc(words * 4));
+  uint32_t* bits = reinterpret_cast<uint32_t*>(count + 4);
+  MALUS_CUDA(cudaMemsetAsync(count, 0, words * 4, stream()));
+  const F16Split sx{x, n, xr.hi, xr.lo, xr.inv, xc.hi, xc.lo, xc.inv, tgt, tdt, V};
+  const F16Split sw = tied ? F16Split{w, V, wv.hi, wv.lo, wv.inv, wd.hi, wd.lo, wd.inv, nullptr, 0, 0}
+                           : F16Split{w, D, wd.hi, wd.lo, wd.inv, wv.hi, wv.lo, wv.inv, nullptr, 0, 0};
+  bool counted = false;
+  if (dw && dx && tied) {
+    const F16Split both[2] = {sx, sw};
+    counted = f16_split_both(both, 2, D, bits, count);
+  } else {
+    if (dw) counted = f16_split_both(&sx, 1, D, bits, count);
+    else f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
+    if (dx) f16_split_both(&sw, 1, tied ? D : V, bits + D, nullptr);
+    else if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
+    else f16_split_cols(sw, V);
+  }
+  if (!counted) xent_count(tgt, tdt, n, V, count);
   // pieces of whole 256-row tiles, of even size
   const bool in_place = xent_rows_in_place(ld);
   const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8))) / 256 * 256);
@@ -86,14 +100,16 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   }
   if (!in_place) scratch_free(planes);
   scratch_free(logits);
+  loss_mean(nll, n, count, loss);
+  scratch_free(count);
 }
 
 void loss_only(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
-               float* nll) {
+               float* nll, float* loss) {
   Planes xr(n, D), wv(V, D);
   f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
   if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
-  else f16_split_cols(w, D, V, wv.hi, wv.lo, wv.inv, nullptr, 0, 0);
+  else f16_split_cols(F16Split{w, D, nullptr, nullptr, nullptr, wv.hi, wv.lo, wv.inv, nullptr, 0, 0}, V);
   const int parts = f16_lse_parts((int)V);
   const int64_t piece = std::min<int64_t>(n, kLossRows);
   float2* part = static_cast<float2*>(scratch_alloc((size_t)piece * (parts * 8 + 4)));
@@ -106,6 +122,7 @@ void loss_only(const float* x, const float* w, const void* tgt, int tdt, bool ti
     xent_join(part, parts, at, t, tdt, V, m, nll + r0);
   }
   scratch_free(part);
+  loss_mean_counted(nll, n, tgt, tdt, V, loss);
 }
 
 // ------------------------------------------------------------- few rows
@@ -396,7 +413,7 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
     return loss;
   }
   const int mode = g_mode.load(std::memory_order_relaxed);
-  if (n && (mode < 0 ? head_small((int64_t)n, (int64_t)D, (int64_t)V) : mode == 1 && n <= 16384)) {
+  if (n && (mode < 0 ? head_small((int64_t)n, (int64_t)D, (int64_t)V, hx || hw) : mode == 1 && n <= 16384)) {
     head_small_run(xp, wp, tp, tdt, tied != 0, (int64_t)n, (int64_t)D, (int64_t)V, fptr(hn), fptr(loss),
                    hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
     if (nll) *nll = hn;
@@ -405,19 +422,15 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
     if (dweight) *dweight = hw;
     return loss;
   }
-  int* count = static_cast<int*>(scratch_alloc(4));
-  xent_count(tp, tdt, (int64_t)n, (int64_t)V, count);
   if (n == 0) {
+    MALUS_CUDA(cudaMemsetAsync(fptr(loss), 0, 4, stream()));
     if (hw) MALUS_CUDA(cudaMemsetAsync(fptr(hw), 0, V * D * 4, stream()));
+  } else if (hx || hw) {
+    train(xp, wp, tp, tdt, tied != 0, (int64_t)n, (int64_t)D, (int64_t)V, ld, fptr(hn), fptr(loss),
+          hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
   } else {
-    const int64_t N = (int64_t)n;
-    if (hx || hw)
-      train(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, ld, count, fptr(hn), hx ? fptr(hx) : nullptr,
-            hw ? fptr(hw) : nullptr);
-    else loss_only(xp, wp, tp, tdt, tied != 0, N, (int64_t)D, (int64_t)V, fptr(hn));
+    loss_only(xp, wp, tp, tdt, tied != 0, (int64_t)n, (int64_t)D, (int64_t)V, fptr(hn), fptr(loss));
   }
-  loss_mean(fptr(hn), (int64_t)n, count, fptr(loss));
-  scratch_free(count);
   if (nll) *nll = hn;
   else tensor_release(hn);
   if (dx) *dx = hx;

@@ -4,10 +4,8 @@
 
 namespace malus {
 
-// Problems of at most this many multiply-adds a product take head_small.cu.
-constexpr double kHeadSmallWork = 2.0e8;
-
-bool head_small(int64_t n, int64_t D, int64_t V);
+// Whether a problem takes f32 multiply-adds (head_small.cu).
+bool head_small(int64_t n, int64_t D, int64_t V, bool grad);
 // loss, nll, and dx and dw where not null.
 void head_small_run(const float* x, const float* w, const void* tgt, int tdt, bool tied, int64_t n, int64_t D, int64_t V,
                     float* nll, float* loss, float* dx, float* dw);

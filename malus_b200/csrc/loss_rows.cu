@@ -226,11 +226,16 @@ __global__ void __launch_bounds__(1024) k_xent_count(const void* __restrict__ tg
   }
 }
 
-// loss = sum of v / max(1, count); with parts, v[r] is first the sum of the row's parts
+// loss = sum of v / max(1, count); with parts, v[r] is first the sum of the row's
+// parts; without count, the rows are counted here by their targets.
 __global__ void __launch_bounds__(1024) k_loss_mean(float* __restrict__ v, const float* __restrict__ part, int parts,
-                                                    int64_t n, const int* __restrict__ count, float* __restrict__ loss) {
+                                                    int64_t n, const int* __restrict__ count, float* __restrict__ loss,
+                                                    const void* __restrict__ tgt, int tdt, int64_t V,
+                                                    int32_t* __restrict__ err) {
   __shared__ double sh[32];
+  __shared__ int shc[32];
   double s = 0.0;
+  int c = 0;
   if (parts) {
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
       float a = 0.0f;
@@ -242,20 +247,39 @@ __global__ void __launch_bounds__(1024) k_loss_mean(float* __restrict__ v, const
   } else {
     for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
       float a[8];
+      int64_t t[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) a[k] = i + k * 1024 < n ? v[i + k * 1024] : 0.0f;
+      for (int k = 0; k < 8; ++k) {
+        const bool in = i + k * 1024 < n;
+        a[k] = in ? v[i + k * 1024] : 0.0f;
+        t[k] = in && tgt ? id_at(tgt, tdt, i + k * 1024) : -1;
+      }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += (double)a[k];
+      for (int k = 0; k < 8; ++k) {
+        s += (double)a[k];
+        c += t[k] >= 0 && t[k] < V;
+        if (t[k] >= V) atomicExch(err, kErrId);
+      }
     }
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+  for (int o = 16; o; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sh[threadIdx.x >> 5] = s;
+    shc[threadIdx.x >> 5] = c;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.0;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) s += sh[i];
-    loss[0] = (float)(s / (double)max(1, count[0]));
+    c = 0;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) {
+      s += sh[i];
+      c += shc[i];
+    }
+    loss[0] = (float)(s / (double)max(1, count ? count[0] : c));
   }
 }
 
@@ -822,7 +846,13 @@ void xent_join(const float2* part, int parts, const float* at, const void* targe
 }
 
 void loss_mean(float* v, int64_t n, const int* count, float* loss) {
-  k_loss_mean<<<1, 1024, 0, stream()>>>(v, nullptr, 0, n, count, loss);
+  k_loss_mean<<<1, 1024, 0, stream()>>>(v, nullptr, 0, n, count, loss, nullptr, 0, 0, nullptr);
+  count_launch();
+  after_launch("k_loss_mean");
+}
+
+void loss_mean_counted(float* v, int64_t n, const void* targets, int tgt_dtype, int64_t V, float* loss) {
+  k_loss_mean<<<1, 1024, 0, stream()>>>(v, nullptr, 0, n, nullptr, loss, targets, tgt_dtype, V, device_error_word());
   count_launch();
   after_launch("k_loss_mean");
 }
@@ -879,7 +909,7 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
     after_launch("k_distill_rows");
     prof_end(pid);
   }
-  k_loss_mean<<<1, 1024, 0, stream()>>>(fptr(hk), part, parts, n, count, fptr(loss));
+  k_loss_mean<<<1, 1024, 0, stream()>>>(fptr(hk), part, parts, n, count, fptr(loss), nullptr, 0, 0, nullptr);
   count_launch();
   after_launch("k_loss_mean");
   scratch_free(ws);

@@ -33,6 +33,10 @@ void xent_join(const float2* part, int parts, const float* at, const void* targe
 // loss[0] = sum of v[0 .. n) / max(1, count[0])
 void loss_mean(float* v, int64_t n, const int* count, float* loss);
 
+// The same, counting the rows whose target lies in [0, V) (and reporting those at or
+// past V).
+void loss_mean_counted(float* v, int64_t n, const void* targets, int tgt_dtype, int64_t V, float* loss);
+
 constexpr int64_t kMaxRowLogits = (int64_t)1 << 24;   // longest row
 
 }  // namespace malus
