@@ -97,12 +97,13 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t tile, bool mn) {
 
 enum Mode : int { kStore = 0, kLse = 1 };
 
-// v times the scales of four columns, which lane `from` holds.
-__device__ __forceinline__ float4 scale4(float4 v, float4 sb4, int from) {
-  v.x *= __shfl_sync(0xffffffffu, sb4.x, from);
-  v.y *= __shfl_sync(0xffffffffu, sb4.y, from);
-  v.z *= __shfl_sync(0xffffffffu, sb4.z, from);
-  v.w *= __shfl_sync(0xffffffffu, sb4.w, from);
+// v times the row's scale and those of four columns, which lane `from` holds.  The
+// scales meet first: each alone may take a sum past the largest float.
+__device__ __forceinline__ float4 scale4(float4 v, float sa, float4 sb4, int from) {
+  v.x *= sa * __shfl_sync(0xffffffffu, sb4.x, from);
+  v.y *= sa * __shfl_sync(0xffffffffu, sb4.y, from);
+  v.z *= sa * __shfl_sync(0xffffffffu, sb4.z, from);
+  v.w *= sa * __shfl_sync(0xffffffffu, sb4.w, from);
   return v;
 }
 
@@ -124,10 +125,8 @@ __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap*
     __syncwarp();
 #pragma unroll
     for (int g = 0; g < 8; ++g) {   // 16-byte granule g of row r lies at g ^ (r & 7): the map's swizzle
-      float4 v = make_float4(acc[c + 4 * g] * sa, acc[c + 4 * g + 1] * sa, acc[c + 4 * g + 2] * sa,
-                             acc[c + 4 * g + 3] * sa);
-      v = scale4(v, sb4, c / 4 + g);
-      mine[g ^ (lane & 7)] = v;
+      mine[g ^ (lane & 7)] = scale4(make_float4(acc[c + 4 * g], acc[c + 4 * g + 1], acc[c + 4 * g + 2], acc[c + 4 * g + 3]),
+                                    sa, sb4, c / 4 + g);
     }
     fence_async_smem();
     __syncwarp();
@@ -144,7 +143,7 @@ __device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols],
   float mx = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kCols; j += 4) {
-    const float4 v = scale4(make_float4(acc[j] * sa, acc[j + 1] * sa, acc[j + 2] * sa, acc[j + 3] * sa), sb4, j / 4);
+    const float4 v = scale4(make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]), sa, sb4, j / 4);
     acc[j] = n0 + j < p.N ? v.x : -INFINITY;
     acc[j + 1] = n0 + j + 1 < p.N ? v.y : -INFINITY;
     acc[j + 2] = n0 + j + 2 < p.N ? v.z : -INFINITY;

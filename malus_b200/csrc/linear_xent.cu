@@ -26,8 +26,6 @@ namespace malus {
 namespace {
 
 constexpr size_t kPieceBytes = (size_t)512 << 20;
-// rows per statistics buffer of the loss alone (8 B per 128 logits)
-constexpr size_t kLossRows = (size_t)1 << 18;
 
 // Half planes of an operand, in one scratch block with their scales.
 struct Planes {
@@ -73,11 +71,13 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
     else f16_split_cols(sw, V);
   }
   if (!counted) xent_count(tgt, tdt, n, V, count);
-  // pieces of whole 256-row tiles, of even size
+  // Pieces of whole 256-row tiles, of even size; of 64 rows (the products' step in K)
+  // where 256 do not fit the bound.
   const bool in_place = xent_rows_in_place(ld);
-  const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8))) / 256 * 256);
+  const int64_t fit = (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8)));
+  const int64_t unit = fit >= 256 ? 256 : 64, most = std::max(unit, fit / unit * unit);
   const int64_t pieces = (n + most - 1) / most;
-  const int64_t piece = ((n + pieces - 1) / pieces + 255) / 256 * 256;
+  const int64_t piece = ((n + pieces - 1) / pieces + unit - 1) / unit * unit;
   float* logits = static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
   float* planes = in_place ? logits : static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
   const __half* hi = reinterpret_cast<const __half*>(planes);
@@ -111,7 +111,8 @@ void loss_only(const float* x, const float* w, const void* tgt, int tdt, bool ti
   if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
   else f16_split_cols(F16Split{w, D, nullptr, nullptr, nullptr, wv.hi, wv.lo, wv.inv, nullptr, 0, 0}, V);
   const int parts = f16_lse_parts((int)V);
-  const int64_t piece = std::min<int64_t>(n, kLossRows);
+  // a piece's statistics (8 B per 128 logits) within the same bound
+  const int64_t piece = std::min<int64_t>(n, std::max<int64_t>(256, (int64_t)(kPieceBytes / ((size_t)parts * 8 + 4))));
   float2* part = static_cast<float2*>(scratch_alloc((size_t)piece * (parts * 8 + 4)));
   float* at = reinterpret_cast<float*>(part + piece * parts);
   for (int64_t r0 = 0; r0 < n; r0 += piece) {

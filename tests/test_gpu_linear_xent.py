@@ -153,6 +153,9 @@ def test_values_of_very_different_scale(M, mode):
     ref, tol = reference(x, w, t)
     for tied in (True, False):
         check(run(M, x, w, t, tied), ref, tol, "scales")
+    # magnitudes whose row scales alone leave the floats' range
+    big, small = (x * np.float32(2.0 ** 100)), (w * np.float32(2.0 ** -100))
+    check(run(M, big, small, t), *reference(big, small, t), "far scales")
     z = np.zeros_like(x)
     loss, nll, dx, dw = run(M, z, w, t)
     assert np.allclose(nll, np.log(300), rtol=1e-6) and not dw.any()
