@@ -8,9 +8,8 @@
 // Bound by HBM: the forward reads x and writes y (8 B per element), the
 // backward reads x and dy and writes dx (12 B).  A row stays in registers
 // between the passes over it (the variance is the two-pass one, of the
-// centred values), held by one warp up to 1024 elements and by a block beyond
-// (up to 16384 elements forward, 8192 backward, where x, dy, w and both column
-// sums take the registers), so each element is read once.  The backward keeps the
+// centred values) up to 8192 elements, held by 8 to 256 threads of a block, so
+// each element is read once.  The backward keeps the
 // same columns in the same thread for all the rows it walks: dw and db grow in
 // registers and leave as one partial row per block, summed in block order
 // by a second kernel (no atomics: the same bits every run).
@@ -21,23 +20,24 @@
 namespace malus {
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Sum of v over the TPR threads of a row (TPR 32: the warp, else the block).
-// `sh` holds one float per warp and alternates between two banks, so one
-// barrier per call is enough.
+// Sum of v over the TPR threads of a row: part of a warp, a warp, or several warps
+// of the block, which then meet at a barrier of their own (group grp's).  `sh`
+// holds one float per warp and alternates between two banks, so one barrier per
+// call is enough.
+constexpr int sh_floats(int tpr) { return tpr > 32 ? 256 / 32 : 1; }
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float (*sh)[TPR / 32], int& bank) {
-  v = warp_sum(v);
+__device__ __forceinline__ float row_sum(float v, float (*sh)[sh_floats(TPR)], int& bank) {
+  constexpr int W = TPR < 32 ? TPR : 32;
+  const int lane = threadIdx.x & 31;
+  const unsigned mask = W == 32 ? 0xffffffffu : ((1u << (W & 31)) - 1u) << (lane & ~(W - 1));
+#pragma unroll
+  for (int o = W / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
   if constexpr (TPR > 32) {
-    float* s = sh[bank];
+    const int grp = threadIdx.x / TPR;
+    float* s = sh[bank] + grp * (TPR / 32);
     bank ^= 1;
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if (lane == 0) s[(threadIdx.x % TPR) >> 5] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(TPR) : "memory");
     v = 0.0f;
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) v += s[i];
@@ -87,14 +87,14 @@ __device__ __forceinline__ void store_row(float* __restrict__ p, int t, int D, c
   }
 }
 
-constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int kBlock = 256;
 
 template <int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(block_of(TPR))
+__global__ void __launch_bounds__(kBlock)
 k_norm_fwd(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
            float* __restrict__ y, float* __restrict__ stats, int64_t rows, int D, float eps) {
-  constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR;
-  __shared__ float sh[2][TPR / 32];
+  constexpr int BLOCK = kBlock, RPB = BLOCK / TPR;
+  __shared__ float sh[2][sh_floats(TPR)];
   int bank = 0;
   const int t = threadIdx.x % TPR;
   const int64_t step = (int64_t)gridDim.x * RPB;
@@ -140,11 +140,11 @@ k_norm_fwd(const float* __restrict__ x, const float* __restrict__ w, const float
 
 // part: [gridDim.x][2][D] partial dw and db (null: neither is wanted); dx may be null.
 template <int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(block_of(TPR))
+__global__ void __launch_bounds__(kBlock)
 k_norm_bwd(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ stats,
            const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ part, int64_t rows, int D) {
-  constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR;
-  __shared__ float sh[2][TPR / 32];
+  constexpr int BLOCK = kBlock, RPB = BLOCK / TPR;
+  __shared__ float sh[2][sh_floats(TPR)];
   extern __shared__ float fold[];   // RPB > 1: [RPB][D], the row groups' partial sums
   int bank = 0;
   const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
@@ -231,23 +231,23 @@ __global__ void __launch_bounds__(1024) k_norm_fold(const float* __restrict__ pa
 }
 
 // Rows longer than a block's registers hold: each pass reads the row again.
-__global__ void __launch_bounds__(512) k_norm_fwd_long(const float* __restrict__ x, const float* __restrict__ w,
+__global__ void __launch_bounds__(kBlock) k_norm_fwd_long(const float* __restrict__ x, const float* __restrict__ w,
                                                        const float* __restrict__ b, float* __restrict__ y,
                                                        float* __restrict__ stats, int64_t rows, int64_t D, float eps) {
-  __shared__ float sh[2][16];
+  __shared__ float sh[2][sh_floats(kBlock)];
   int bank = 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float* xr = x + r * D;
     float s = 0.0f;
-    for (int64_t c = threadIdx.x; c < D; c += 512) s += xr[c];
-    const float mean = row_sum<512>(s, sh, bank) / (float)D;
+    for (int64_t c = threadIdx.x; c < D; c += kBlock) s += xr[c];
+    const float mean = row_sum<kBlock>(s, sh, bank) / (float)D;
     float q = 0.0f;
-    for (int64_t c = threadIdx.x; c < D; c += 512) {
+    for (int64_t c = threadIdx.x; c < D; c += kBlock) {
       const float d = xr[c] - mean;
       q += d * d;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<512>(q, sh, bank) / (float)D + eps);
-    for (int64_t c = threadIdx.x; c < D; c += 512) {
+    const float rstd = 1.0f / sqrtf(row_sum<kBlock>(q, sh, bank) / (float)D + eps);
+    for (int64_t c = threadIdx.x; c < D; c += kBlock) {
       float v = (xr[c] - mean) * rstd;
       if (w) v *= w[c];
       if (b) v += b[c];
@@ -260,23 +260,23 @@ __global__ void __launch_bounds__(512) k_norm_fwd_long(const float* __restrict__
   }
 }
 
-__global__ void __launch_bounds__(512) k_norm_dx_long(const float* __restrict__ x, const float* __restrict__ w,
+__global__ void __launch_bounds__(kBlock) k_norm_dx_long(const float* __restrict__ x, const float* __restrict__ w,
                                                       const float* __restrict__ stats, const float* __restrict__ dy,
                                                       float* __restrict__ dx, int64_t rows, int64_t D) {
-  __shared__ float sh[2][16];
+  __shared__ float sh[2][sh_floats(kBlock)];
   int bank = 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float *xr = x + r * D, *gr = dy + r * D;
     const float mean = stats[2 * r], rstd = stats[2 * r + 1];
     float s = 0.0f, sx = 0.0f;
-    for (int64_t c = threadIdx.x; c < D; c += 512) {
+    for (int64_t c = threadIdx.x; c < D; c += kBlock) {
       const float g = gr[c] * (w ? w[c] : 1.0f);
       s += g;
       sx += g * ((xr[c] - mean) * rstd);
     }
-    const float ms = row_sum<512>(s, sh, bank) / (float)D;
-    const float msx = row_sum<512>(sx, sh, bank) / (float)D;
-    for (int64_t c = threadIdx.x; c < D; c += 512) {
+    const float ms = row_sum<kBlock>(s, sh, bank) / (float)D;
+    const float msx = row_sum<kBlock>(sx, sh, bank) / (float)D;
+    for (int64_t c = threadIdx.x; c < D; c += kBlock) {
       const float g = gr[c] * (w ? w[c] : 1.0f);
       dx[r * D + c] = ((g - ms) - (xr[c] - mean) * rstd * msx) * rstd;
     }
@@ -305,18 +305,27 @@ bool aligned16(std::initializer_list<const void*> ps) {
   return (a & 15) == 0;
 }
 
-constexpr int64_t kMaxFwd = 16384, kMaxBwd = 8192;   // longest rows held in registers
+constexpr int kFwdNv = 8, kBwdNv = 4;
+constexpr int64_t kMaxRow = 8192;   // longest row held in registers
 
-// Threads per row: a warp holds 1024 elements, a block of 256 holds 8192, one
-// of 512 holds 16384; `nv` float4 groups of each thread cover the row.
+// Threads per row, and the float4 groups `nv` that each holds.  Few threads for short
+// rows (200000 x 96 forward: 29 us with 8 threads a row, 51 with 32), up to `most`
+// groups each; a warp up to 1024 elements; beyond, up to 6 groups each (16384 x 1281
+// forward: 38 us with 64 threads, 56 with 256; but 8192 x 2048: 32 with 64 threads
+// and 8 groups, 27 with 256 and 2) until 256 threads hold 8.
 struct RowCfg { int tpr, nv; };
-RowCfg row_cfg(int64_t D) {
-  const int tpr = D <= 1024 ? 32 : D <= 8192 ? 256 : 512;
+RowCfg row_cfg(int64_t D, int most) {
+  int tpr = 8;
+  while (tpr < 32 && D > 4 * most * tpr) tpr *= 2;
+  if (D > 1024)
+    for (tpr = 64; tpr < 256 && D > 4 * 6 * tpr;) tpr *= 2;
   return {tpr, (int)((D + 4 * tpr - 1) / (4 * tpr))};
 }
 
+// 64 and 128 threads never hold more than 6 groups each.
 template <int TPR, bool VEC, class F>
 void with_nv(int nv, F&& f) {
+  constexpr int kMost = TPR == 64 || TPR == 128 ? 6 : 8;
   switch (nv) {
     case 1: f.template operator()<TPR, 1, VEC>(); break;
     case 2: f.template operator()<TPR, 2, VEC>(); break;
@@ -324,14 +333,25 @@ void with_nv(int nv, F&& f) {
     case 4: f.template operator()<TPR, 4, VEC>(); break;
     case 5: f.template operator()<TPR, 5, VEC>(); break;
     case 6: f.template operator()<TPR, 6, VEC>(); break;
-    case 7: f.template operator()<TPR, 7, VEC>(); break;
-    default: f.template operator()<TPR, 8, VEC>(); break;
+    case 7: f.template operator()<TPR, std::min(7, kMost), VEC>(); break;
+    default: f.template operator()<TPR, std::min(8, kMost), VEC>(); break;
+  }
+}
+template <bool VEC, class F>
+void with_tpr(RowCfg c, F&& f) {
+  switch (c.tpr) {
+    case 8: with_nv<8, VEC>(c.nv, f); break;
+    case 16: with_nv<16, VEC>(c.nv, f); break;
+    case 32: with_nv<32, VEC>(c.nv, f); break;
+    case 64: with_nv<64, VEC>(c.nv, f); break;
+    case 128: with_nv<128, VEC>(c.nv, f); break;
+    default: with_nv<256, VEC>(c.nv, f); break;
   }
 }
 template <class F>
 void with_cfg(RowCfg c, bool vec, F&& f) {
-  if (c.tpr == 32) vec ? with_nv<32, true>(c.nv, f) : with_nv<32, false>(c.nv, f);
-  else vec ? with_nv<256, true>(c.nv, f) : with_nv<256, false>(c.nv, f);
+  if (vec) with_tpr<true>(c, f);
+  else with_tpr<false>(c, f);
 }
 
 struct FwdLaunch {
@@ -342,7 +362,7 @@ struct FwdLaunch {
   float eps;
   template <int TPR, int NV, bool VEC>
   void operator()() const {
-    constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR;
+    constexpr int BLOCK = kBlock, RPB = BLOCK / TPR;
     const int64_t need = (rows + RPB - 1) / RPB;
     const unsigned grid = (unsigned)std::min<int64_t>(need, (int64_t)kNumSMs * (2048 / BLOCK));
     k_norm_fwd<TPR, NV, VEC><<<grid, BLOCK, 0, stream()>>>(x, w, b, y, stats, rows, D, eps);
@@ -356,7 +376,7 @@ struct BwdLaunch {
   int D;
   template <int TPR, int NV, bool VEC>
   void operator()() const {
-    constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR;
+    constexpr int BLOCK = kBlock, RPB = BLOCK / TPR;
     const int64_t need = (rows + RPB - 1) / RPB;
     // one resident wave: every block leaves one partial row
     static int per_sm = [] {
@@ -384,15 +404,13 @@ void norm_affine_fwd(const float* x, const float* w, const float* b, float* y, f
                      int64_t D, float eps) {
   if (rows == 0) return;
   const int pid = prof_begin_named("k_norm_fwd", 4.0 * (2.0 * rows * D + 2.0 * D));
-  if (D > kMaxFwd) {
-    k_norm_fwd_long<<<(unsigned)std::min<int64_t>(rows, kNumSMs * 4), 512, 0, stream()>>>(x, w, b, y, stats, rows, D,
+  if (D > kMaxRow) {
+    k_norm_fwd_long<<<(unsigned)std::min<int64_t>(rows, kNumSMs * 8), kBlock, 0, stream()>>>(x, w, b, y, stats, rows, D,
                                                                                          eps);
   } else {
     const bool vec = D % 4 == 0 && aligned16({x, w, b, y});
     const FwdLaunch f{x, w, b, y, stats, rows, (int)D, eps};
-    const RowCfg c = row_cfg(D);
-    if (c.tpr == 512) vec ? with_nv<512, true>(c.nv, f) : with_nv<512, false>(c.nv, f);
-    else with_cfg(c, vec, f);
+    with_cfg(row_cfg(D, kFwdNv), vec, f);
   }
   count_launch();
   after_launch("k_norm_fwd");
@@ -407,9 +425,9 @@ void norm_affine_bwd(const float* x, const float* w, const float* stats, const f
     return;
   }
   const int pid = prof_begin_named("k_norm_bwd", 4.0 * ((dx ? 3.0 : 2.0) * rows * D + 3.0 * D));
-  if (D > kMaxBwd) {
+  if (D > kMaxRow) {
     if (dx) {
-      k_norm_dx_long<<<(unsigned)std::min<int64_t>(rows, kNumSMs * 4), 512, 0, stream()>>>(x, w, stats, dy, dx, rows, D);
+      k_norm_dx_long<<<(unsigned)std::min<int64_t>(rows, kNumSMs * 8), kBlock, 0, stream()>>>(x, w, stats, dy, dx, rows, D);
       count_launch();
     }
     if (dw || db) {
@@ -422,7 +440,7 @@ void norm_affine_bwd(const float* x, const float* w, const float* stats, const f
     }
   } else {
     const bool vec = D % 4 == 0 && aligned16({x, w, dy, dx});
-    with_cfg(row_cfg(D), vec, BwdLaunch{x, w, stats, dy, dx, dw, db, rows, (int)D});
+    with_cfg(row_cfg(D, kBwdNv), vec, BwdLaunch{x, w, stats, dy, dx, dw, db, rows, (int)D});
     count_launch();
   }
   after_launch("k_norm_bwd");
