@@ -315,15 +315,18 @@ k_head_few_end(const float2* __restrict__ part, int parts, const float* __restri
     const int64_t t = target_at(tgt, tdt, i);
     counted = t >= 0 && t < V;
     if (t >= V && lane == 0) atomicExch(err, 4);
-    Run r;
-    for (int k = lane; k < parts; k += 32) {
-      const float2 o = part[(int64_t)i * parts + k];
-      r.join(o.x, o.y);
-    }
+    const float2* p = part + (int64_t)i * parts;
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+    for (int k = lane; k < parts; k += 32) m = fmaxf(m, p[k].x);
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      r.join(__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o));
-    if (counted) v = logf(r.s) - (at[i] - r.m);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll 8
+    for (int k = lane; k < parts; k += 32) sum += p[k].y * exp2f((p[k].x - m0) * kLog2e);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (counted) v = logf(sum) - (at[i] - m);
     if (lane == 0) nll[i] = v;
   }
   if (lane == 0) sh[i] = v;
