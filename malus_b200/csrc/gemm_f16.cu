@@ -11,8 +11,8 @@
 // with products of known sums: a chain of n additions loses about n * 2e-8 of
 // the magnitude, all in one direction; K = 50304 as one chain is off by 8e-5).
 // So a chain is kept short: within a 64-deep stage the small cross products come
-// first, then the four hi*hi additions, and after every fourth stage (K = 256)
-// the epilogue warps take the accumulator out of tensor memory and add it,
+// first, then the four hi*hi additions, and after every fourth stage (K = 256; every
+// second in short units) the epilogue warps take the accumulator out of tensor memory and add it,
 // rounding to nearest, to sums in their registers, while the tensor core fills
 // the other accumulator.
 //
@@ -35,7 +35,9 @@ using namespace malus::tc;
 constexpr int BM = 128, BN = 256, BK = 64, STAGES = 3;
 constexpr int kTile = 128 * BK * 2;                 // one plane's 128 rows, 64 deep
 constexpr int kStageBytes = 4 * kTile;              // A hi, A lo, B hi, B lo
-constexpr int kChunk = 4;                           // stages per accumulator
+// Stages per accumulator, and for units short enough that the pipeline's latency
+// and not its rate decides (one unit of at most kShortUnit stages per pair).
+constexpr int kChunk = 4, kShortChunk = 2, kShortUnit = 16;
 constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
 constexpr int kCols = BN * 4 / kEpiWarps;           // columns of a row that an epilogue thread holds
 // Registers per thread: 168 at launch; the warpgroup of the TMA and MMA warps
@@ -49,6 +51,7 @@ static_assert(kSmem <= 232448 && kCols == 128, "shared memory; a warp's lanes ho
 
 struct Params {
   int M, N, K, tiles_m, tiles_n, nst, splits;
+  int chunk;           // stages per accumulator
   int a_mn, b_mn;
   int64_t a_k0, b_k0;
   const float *a_inv, *b_inv;
@@ -270,7 +273,7 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
       bool ok = true, issued = false;
       for (int u = grp; u < total && ok; u += ngrp) {
         const Unit un = unit_at(p, u);
-        for (int st = un.st_lo; st < un.st_hi && ok; st += kChunk, ++chunk) {
+        for (int st = un.st_lo; st < un.st_hi && ok; st += p.chunk, ++chunk) {
           const uint32_t b = chunk & 1, v = chunk >> 1;
           if (v >= 1 && !mbar_wait_cluster(smem_u32(&acce[b]), (v - 1) & 1, abort_flag, p.err, 44)) {
             ok = false;
@@ -278,7 +281,7 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t dacc = tmem + b * BN;
-          const int end = min(st + kChunk, un.st_hi);
+          const int end = min(st + p.chunk, un.st_hi);
           for (int q = st; q < end; ++q, ++it) {
             const int s = it % STAGES;
             if (!mbar_wait(smem_u32(&full[s]), (it / STAGES) & 1, abort_flag, p.err, 42)) {
@@ -329,7 +332,7 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
       const float4 sb4 = p.b_inv ? *reinterpret_cast<const float4*>(p.b_inv + n0 + 4 * lane)
                                  : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
       float acc[kCols];
-      for (int st = un.st_lo; st < un.st_hi; st += kChunk, ++chunk) {
+      for (int st = un.st_lo; st < un.st_hi; st += p.chunk, ++chunk) {
         const uint32_t b = chunk & 1;
         if (!mbar_wait(smem_u32(&accf[b]), (chunk >> 1) & 1, abort_flag, p.err, 43)) {
           ok = false;
@@ -739,6 +742,9 @@ void launch(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstrid
   p.inv_all = (g.a.inv ? 1.0f : g.a.inv_all) * (g.b.inv ? 1.0f : g.b.inv_all);
   p.err = device_error_word();
   const int units = p.tiles_m * p.tiles_n * p.splits;
+  // half the chain where it costs nothing (16384 x 384 x 65, three products: 60 us
+  // either way; 2048 x 768 x 50304: 377 us with 4, 472 with 2)
+  p.chunk = units <= max_pairs() && (p.nst + p.splits - 1) / p.splits <= kShortUnit ? kShortChunk : kChunk;
   cudaLaunchAttribute at[1];
   cudaLaunchConfig_t cfg = config<MODE>(2 * std::min(units, max_pairs()), at);
   CUtensorMap mo = {};
