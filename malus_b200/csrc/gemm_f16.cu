@@ -1,9 +1,12 @@
 // f32 GEMM on the half-precision tensor pipe.
 //
 // Each operand row is scaled by a power of two and split into two halves, hi =
-// half_rn(x), lo = half_rn(x - hi): 22 bits of every element within 2^-18 of its
-// row's largest, and an error of at most 2^-40 of that largest for smaller
-// ones.  The product keeps hi*lo + lo*hi + hi*hi (the dropped lo*lo is below
+// half_rn(x), lo = half_rn(x - hi): 22 bits of every element within 2^-16 of its
+// row's largest, and an error of at most 2^-38 of that largest for smaller ones
+// (the largest is brought to 2^13 or more, where half's grid of 2^-24 rounds by
+// 2^-25).  An operand may have a scale per 256 of K and row instead, applied as each
+// accumulator is added to the sums: then "its row's largest" is that of the 256.
+// The product keeps hi*lo + lo*hi + hi*hi (the dropped lo*lo is below
 // 2^-22 of a term).  Against three tf32 products of the same 22 bits this takes
 // half the tensor time and half the operand bytes.
 //
@@ -52,9 +55,12 @@ static_assert(kSmem <= 232448 && kCols == 128, "shared memory; a warp's lanes ho
 struct Params {
   int M, N, K, tiles_m, tiles_n, nst, splits;
   int chunk;           // stages per accumulator
-  int a_mn, b_mn;
+  int align;           // K slices start at multiples of so many stages
+  int a_mn, b_mn, a_grouped;
   int64_t a_k0, b_k0;
   const float *a_inv, *b_inv;
+  const float* block_inv;   // of A (kByM) or of B (kByN)
+  int64_t block_pitch;
   float inv_all;
   int accumulate;
   const int* count;
@@ -75,8 +81,9 @@ __device__ __forceinline__ Unit unit_at(const Params& p, int u) {
   const int j = p.inner_m ? tile / p.tiles_m : tile % p.tiles_n;
   r.m0 = i * 2 * BM;
   r.n0 = j * BN;
-  r.st_lo = (int)((int64_t)r.split * p.nst / p.splits);
-  r.st_hi = (int)((int64_t)(r.split + 1) * p.nst / p.splits);
+  const int64_t steps = (p.nst + p.align - 1) / p.align;
+  r.st_lo = (int)(r.split * steps / p.splits) * p.align;
+  r.st_hi = min((int)((r.split + 1) * steps / p.splits) * p.align, p.nst);
   return r;
 }
 
@@ -98,7 +105,9 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t tile, bool mn) {
   return mn ? umma_desc(tile, BK * 128, 1024, 2) : umma_desc(tile, 16, 1024, 2);
 }
 
-enum Mode : int { kStore = 0, kLse = 1 };
+// What becomes of the sums: stored; row statistics; both; stored, with A's or B's
+// scales (which change from chunk to chunk) applied to each chunk as it is added.
+enum Mode : int { kStore = 0, kLse = 1, kBoth = 2, kByM = 3, kByN = 4 };
 
 // v times the row's scale and those of four columns, which lane `from` holds.  The
 // scales meet first: each alone may take a sum past the largest float.
@@ -115,7 +124,8 @@ __device__ __forceinline__ float4 scale4(float4 v, float sa, float4 sb4, int fro
 // scaled and sent to the output 32 columns at a time through the warp's staging
 // block, which a TMA store (or, accumulating, a TMA add: one per element and
 // launch, so the order is fixed) takes from there.  The copy drops what lies
-// past M or N.
+// past M or N.  SCALED: acc has its scales already.
+template <bool SCALED>
 __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap* mOut, const Unit& un,
                                              float (&acc)[kCols], int m0, int n0, float sa, float4 sb4, uint8_t* stage) {
   const int lane = threadIdx.x & 31;
@@ -128,8 +138,8 @@ __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap*
     __syncwarp();
 #pragma unroll
     for (int g = 0; g < 8; ++g) {   // 16-byte granule g of row r lies at g ^ (r & 7): the map's swizzle
-      mine[g ^ (lane & 7)] = scale4(make_float4(acc[c + 4 * g], acc[c + 4 * g + 1], acc[c + 4 * g + 2], acc[c + 4 * g + 3]),
-                                    sa, sb4, c / 4 + g);
+      const float4 v = make_float4(acc[c + 4 * g], acc[c + 4 * g + 1], acc[c + 4 * g + 2], acc[c + 4 * g + 3]);
+      mine[g ^ (lane & 7)] = SCALED ? v : scale4(v, sa, sb4, c / 4 + g);
     }
     fence_async_smem();
     __syncwarp();
@@ -141,7 +151,8 @@ __device__ __forceinline__ void finish_store(const Params& p, const CUtensorMap*
   }
 }
 
-// The sums of a row into its maximum, sum of exponentials and target value.
+// The sums of a row into its maximum, sum of exponentials and target value; acc is
+// scaled after it (-inf past N).
 __device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols], int m, int n0, float sa, float4 sb4) {
   float mx = -INFINITY;
 #pragma unroll
@@ -238,8 +249,11 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
           if (rank == 0) mbar_expect_tx(fb, 2 * kStageBytes);   // this CTA's and rank 1's copies
           fb = cluster_addr(fb, 0);
           const int ka = (int)p.a_k0 + st * BK, kb = (int)p.b_k0 + st * BK;
-          // K-major boxes are 64 (K) x 128 rows; MN-major boxes 64 columns x 64 (K) x 2 column chunks
-          const int a0 = p.a_mn ? 0 : ka, a1 = p.a_mn ? ka : m0, a2 = p.a_mn ? m0 >> 6 : 0;
+          // K-major boxes are 64 (K) x 128 rows, grouped ones 64 x 1 group x 128 rows; MN-major
+          // boxes 64 columns x 64 (K) x 2 column chunks
+          const int a0 = p.a_mn || p.a_grouped ? 0 : ka;
+          const int a1 = p.a_mn ? ka : p.a_grouped ? ka >> 6 : m0;
+          const int a2 = p.a_mn ? m0 >> 6 : p.a_grouped ? m0 : 0;
           const int b0 = p.b_mn ? 0 : kb, b1 = p.b_mn ? kb : n0, b2 = p.b_mn ? n0 >> 6 : 0;
           tma_load_3d_pair(smem_u32(sp), &mAh, fb, a0, a1, a2);
           tma_load_3d_pair(smem_u32(sp + kTile), &mAl, fb, a0, a1, a2);
@@ -334,12 +348,35 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
       float acc[kCols];
       for (int st = un.st_lo; st < un.st_hi; st += p.chunk, ++chunk) {
         const uint32_t b = chunk & 1;
+        // the chunk's scales, on their way while its sums come in
+        const float* block = MODE == kByM || MODE == kByN
+                                 ? p.block_inv + (int64_t)(st / (kF16Block / BK)) * p.block_pitch : nullptr;
+        const float bm = MODE == kByM ? block[m0 + lane] : 1.0f;
+        const float4 bn = MODE == kByN ? *reinterpret_cast<const float4*>(block + n0 + 4 * lane)
+                                       : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
         if (!mbar_wait(smem_u32(&accf[b]), (chunk >> 1) & 1, abort_flag, p.err, 43)) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (st == un.st_lo) {
+        if constexpr (MODE == kByM || MODE == kByN) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(tbase + b * BN + c, r);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              float4 s = make_float4(bm, bm, bm, bm);
+              if (MODE == kByN) s = scale4(make_float4(1.0f, 1.0f, 1.0f, 1.0f), 1.0f, bn, (c + j) / 4);
+              float* a = acc + c + j;
+              const bool first = st == un.st_lo;
+              a[0] = fmaf(__uint_as_float(r[j]), s.x, first ? 0.0f : a[0]);
+              a[1] = fmaf(__uint_as_float(r[j + 1]), s.y, first ? 0.0f : a[1]);
+              a[2] = fmaf(__uint_as_float(r[j + 2]), s.z, first ? 0.0f : a[2]);
+              a[3] = fmaf(__uint_as_float(r[j + 3]), s.w, first ? 0.0f : a[3]);
+            }
+          }
+        } else if (st == un.st_lo) {
 #pragma unroll
           for (int c = 0; c < kCols; c += 32) tmem_ld32(tbase + b * BN + c, reinterpret_cast<uint32_t*>(acc + c));
         } else {
@@ -356,11 +393,12 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
         if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acce[b]), 0));
       }
       if (!ok) break;
-      if (MODE == kLse) finish_lse(p, acc, m0 + lane, n0, sa, sb4);
-      else finish_store(p, &mOut, un, acc, m0, n0, sa, sb4, stage);
+      if (MODE == kLse || MODE == kBoth) finish_lse(p, acc, m0 + lane, n0, sa, sb4);
+      if (MODE == kBoth) __syncwarp();
+      if (MODE != kLse) finish_store<MODE == kBoth>(p, &mOut, un, acc, m0, n0, sa, sb4, stage);
       __syncwarp();   // rows past M return early: the next tensor memory load needs the whole warp
     }
-    if (MODE == kStore && lane == 0) bulk_wait<0>();   // every copy is done before the CTA exits
+    if (MODE != kLse && lane == 0) bulk_wait<0>();   // every copy is done before the CTA exits
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(done));
@@ -409,24 +447,6 @@ __global__ void __launch_bounds__(256) k_f16_join(const float* __restrict__ ws, 
 }
 
 // ------------------------------------------------------------------ planes
-// The power of two that brings `m` (a magnitude, its bits) into [2^13, 2^14), as
-// a scale and its inverse; 1 for zero.  Both stay normal numbers.
-__device__ __forceinline__ void scale_for(uint32_t bits, float* up, float* inv) {
-  int e = (int)(bits >> 23) - 127;              // floor(log2), -127 for subnormals
-  int s = bits ? kF16Exp - e : 0;
-  s = s > 126 ? 126 : s < -113 ? -113 : s;
-  *up = __uint_as_float((uint32_t)(s + 127) << 23);
-  *inv = __uint_as_float((uint32_t)(127 - s) << 23);
-}
-__device__ __forceinline__ uint32_t finite_bits(float x) {   // bits of |x|; 0 for inf and NaN
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b >= 0x7f800000u ? 0u : b;
-}
-__device__ __forceinline__ void split2(float x, __half* h, __half* l) {
-  *h = __float2half_rn(x);
-  *l = __float2half_rn(x - __half2float(*h));
-}
-
 // One row per group of G threads (a warp, or a block of 512).
 template <int G, bool VEC>
 __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* __restrict__ src, int64_t R, int64_t C,
@@ -441,10 +461,10 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* _
     if (VEC) {
       for (int64_t c = 4 * t; c < C; c += 4 * G) {
         const float4 v = *reinterpret_cast<const float4*>(s + c);
-        m = max(m, max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w))));
+        m = max(m, max(max(f16_finite_bits(v.x), f16_finite_bits(v.y)), max(f16_finite_bits(v.z), f16_finite_bits(v.w))));
       }
     } else {
-      for (int64_t c = t; c < C; c += G) m = max(m, finite_bits(s[c]));
+      for (int64_t c = t; c < C; c += G) m = max(m, f16_finite_bits(s[c]));
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (G > 32) {
@@ -454,7 +474,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* _
       __syncthreads();
     }
     float up, iv;
-    scale_for(m, &up, &iv);
+    f16_scale(m, &up, &iv);
     if (t == 0) inv[r] = iv;
     __half *hr = hi + r * Cp, *lr = lo + r * Cp;
     for (int64_t c = 4 * t; c < Cp; c += 4 * G) {
@@ -468,7 +488,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) k_split_rows(const float* _
       }
       __align__(8) __half h[4], l[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split2(v[j] * up, &h[j], &l[j]);
+      for (int j = 0; j < 4; ++j) f16_split(v[j] * up, &h[j], &l[j]);
       *reinterpret_cast<uint2*>(hr + c) = *reinterpret_cast<uint2*>(h);
       *reinterpret_cast<uint2*>(lr + c) = *reinterpret_cast<uint2*>(l);
     }
@@ -535,13 +555,13 @@ __global__ void __launch_bounds__(512, 1) k_split_rows_max(const SplitJobs jobs,
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < 4 * NV; ++k) {
-      const uint32_t b = finite_bits(v[k]);
+      const uint32_t b = f16_finite_bits(v[k]);
       m = max(m, b);
       cm[k] = max(cm[k], in ? b : 0u);
     }
     m = __reduce_max_sync(0xffffffffu, m);
     float up, iv;
-    scale_for(m, &up, &iv);
+    f16_scale(m, &up, &iv);
     if (lane == 0) inv[r] = iv;
     __half *hr = hi + r * Cp, *lr = lo + r * Cp;
 #pragma unroll
@@ -550,7 +570,7 @@ __global__ void __launch_bounds__(512, 1) k_split_rows_max(const SplitJobs jobs,
       if (i < Cp) {
         __align__(8) __half h[4], l[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split2(v[4 * k + j] * up, &h[j], &l[j]);
+        for (int j = 0; j < 4; ++j) f16_split(v[4 * k + j] * up, &h[j], &l[j]);
         *reinterpret_cast<uint2*>(hr + i) = *reinterpret_cast<uint2*>(h);
         *reinterpret_cast<uint2*>(lr + i) = *reinterpret_cast<uint2*>(l);
       }
@@ -599,7 +619,7 @@ __global__ void __launch_bounds__(256) k_col_max(const float* __restrict__ src, 
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) m[j] = max(m[j], k[i] ? finite_bits(v[i][j]) : 0u);
+        for (int j = 0; j < W; ++j) m[j] = max(m[j], k[i] ? f16_finite_bits(v[i][j]) : 0u);
     }
   }
 #pragma unroll
@@ -653,7 +673,7 @@ __global__ void __launch_bounds__(256) k_split_cols(const SplitJobs jobs, int64_
     const uint32_t b = __ballot_sync(0xffffffffu, k);
     if ((t & 31) == 0) rows_kept[t >> 5] = b;
     float up = 1.0f, iv = 1.0f;
-    if (t < nc) scale_for(bits[c0 + t], &up, &iv);
+    if (t < nc) f16_scale(bits[c0 + t], &up, &iv);
     ups[t] = up;
     if (rt == 0 && t < nc) job.cinv[c0 + t] = iv;
   }
@@ -671,7 +691,7 @@ __global__ void __launch_bounds__(256) k_split_cols(const SplitJobs jobs, int64_
     const float up = ups[c];
     __align__(8) __half h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split2(k4 >> k & 1 ? tile[r + k][c] * up : 0.0f, &h[k], &l[k]);
+    for (int k = 0; k < 4; ++k) f16_split(k4 >> k & 1 ? tile[r + k][c] * up : 0.0f, &h[k], &l[k]);
     *reinterpret_cast<uint2*>(h0 + c * Rp) = *reinterpret_cast<uint2*>(h);
     *reinterpret_cast<uint2*>(l0 + c * Rp) = *reinterpret_cast<uint2*>(l);
   }
@@ -681,8 +701,14 @@ __global__ void __launch_bounds__(256) k_split_cols(const SplitJobs jobs, int64_
 CUtensorMap map_of(const F16Operand& o, const __half* plane) {
   const uint64_t pb = (uint64_t)o.pitch * 2;
   if (o.mn_major) {
-    const uint64_t dims[3] = {64, (uint64_t)o.rows, (uint64_t)(o.cols + 63) / 64}, st[2] = {pb, 128};
+    const uint64_t dims[3] = {64, (uint64_t)o.rows, (uint64_t)(o.cols + 63) / 64};
+    const uint64_t st[2] = {pb, (uint64_t)(o.grouped ? 256 : 128)};
     const uint32_t box[3] = {64, BK, 2};
+    return encode_f16_map(3, plane, dims, st, box);
+  }
+  if (o.grouped) {
+    const uint64_t dims[3] = {64, (uint64_t)(o.cols + 63) / 64, (uint64_t)o.rows}, st[2] = {256, pb};
+    const uint32_t box[3] = {64, 1, 128};
     return encode_f16_map(3, plane, dims, st, box);
   }
   const uint64_t dims[3] = {(uint64_t)o.cols, (uint64_t)o.rows, 1}, st[2] = {pb, pb * (uint64_t)o.rows};
@@ -737,6 +763,7 @@ void launch(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstrid
   p.tiles_n = (g.N + BN - 1) / BN;
   p.inner_m = p.tiles_m <= p.tiles_n;
   p.a_mn = g.a.mn_major; p.b_mn = g.b.mn_major;
+  p.a_grouped = g.a.grouped;
   p.a_k0 = g.a.k0; p.b_k0 = g.b.k0;
   p.a_inv = g.a.inv; p.b_inv = g.b.inv;
   p.inv_all = (g.a.inv ? 1.0f : g.a.inv_all) * (g.b.inv ? 1.0f : g.b.inv_all);
@@ -745,10 +772,12 @@ void launch(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstrid
   // half the chain where it costs nothing (16384 x 384 x 65, three products: 60 us
   // either way; 2048 x 768 x 50304: 377 us with 4, 472 with 2)
   p.chunk = units <= max_pairs() && (p.nst + p.splits - 1) / p.splits <= kShortUnit ? kShortChunk : kChunk;
+  // a chunk lies within one block of scales
+  p.align = MODE == kByM || MODE == kByN ? p.chunk : 1;
   cudaLaunchAttribute at[1];
   cudaLaunchConfig_t cfg = config<MODE>(2 * std::min(units, max_pairs()), at);
   CUtensorMap mo = {};
-  if (MODE == kStore) {
+  if (MODE != kLse) {
     const uint64_t dims[3] = {(uint64_t)g.N, (uint64_t)g.M, (uint64_t)p.splits};
     const uint64_t st[2] = {(uint64_t)ldo * 4, (uint64_t)sstride * 4};
     const uint32_t box[3] = {32, 32, 1};
@@ -779,6 +808,16 @@ int splits_for(int tiles, int nst, int pairs) {
 
 }  // namespace
 
+static void launch_store(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstride) {
+  static_assert(kF16Block % (kChunk * BK) == 0 && kChunk % kShortChunk == 0, "a chunk crosses no block of scales");
+  const F16Operand& s = g.a.block_inv ? g.a : g.b;
+  p.block_inv = s.block_inv;
+  p.block_pitch = s.block_pitch;
+  if (g.a.block_inv) launch<kByM>(g, p, out, ldo, sstride);
+  else if (g.b.block_inv) launch<kByN>(g, p, out, ldo, sstride);
+  else launch<kStore>(g, p, out, ldo, sstride);
+}
+
 void gemm_f16(const F16Gemm& g) {
   if (g.M <= 0 || g.N <= 0) return;
   if (g.K <= 0) panic("gemm_f16 with K = %d", g.K);
@@ -789,13 +828,13 @@ void gemm_f16(const F16Gemm& g) {
   p.count = g.count;
   if (p.splits == 1 && g.ldo % 4 == 0 && ((uintptr_t)g.out & 15) == 0) {
     p.accumulate = g.accumulate;
-    launch<kStore>(g, p, g.out, g.ldo, (int64_t)g.M * g.ldo);
+    launch_store(g, p, g.out, g.ldo, (int64_t)g.M * g.ldo);
     return;
   }
   // K slices, or rows that a TMA store cannot address: through a workspace
   const int64_t ldw = ((int64_t)g.N + 3) / 4 * 4, sstride = (int64_t)g.M * ldw;
   float* ws = static_cast<float*>(scratch_alloc((size_t)sstride * p.splits * 4));
-  launch<kStore>(g, p, ws, ldw, sstride);
+  launch_store(g, p, ws, ldw, sstride);
   const unsigned gx = (unsigned)((g.N + 1023) / 1024);
   for (int m0 = 0; m0 < g.M; m0 += 65535) {
     const dim3 grid(gx, (unsigned)std::min(65535, g.M - m0));
@@ -821,7 +860,8 @@ void gemm_f16_lse(const F16Gemm& g, float2* part, float* at, const void* target,
   p.at = at;
   p.target = target;
   p.tdt = tgt_dtype;
-  launch<kLse>(g, p, nullptr, 0, 0);
+  if (g.out) launch<kBoth>(g, p, g.out, g.ldo, (int64_t)g.M * g.ldo);
+  else launch<kLse>(g, p, nullptr, 0, 0);
 }
 
 void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv) {

@@ -4,13 +4,18 @@
 //   logits = x W^T,  nll = logsumexp(logits) - logits[target]
 //   dl = (softmax(logits) - onehot(target)) / rows,  dx = dl W,  dW = dl^T x
 //
-// Training takes the tokens in pieces: a piece's logits live in a scratch of at
-// most kPieceBytes, become the half planes of dl in place (loss_rows.cu), feed
-// both gradient products and make room for the next piece.  That is the three
-// products (6 N D V flops) and nothing computed twice; the scratch costs 4 B
-// written and read per logit, then 4 B written and read by each product.  The
-// loss alone stores no logits: the product's epilogue reduces each row of a tile
-// to its maximum, sum of exponentials and target logit.
+// Training takes the tokens in pieces: a piece's logits become half planes of dl
+// (loss_rows.cu), feed both gradient products and make room for the next piece.
+// That is the three products (6 N D V flops) and nothing computed twice.  dx and
+// dweight each have planes of their own: dx sums over the vocabulary, where one scale
+// serves; dweight sums over the tokens, and there each entry's gradients are scaled
+// by their own largest, so that the row of a token that is hardly ever predicted is
+// as accurate as any other.  A piece holds at most kPieceBytes of logits (or 64 rows
+// of them, which is more from V = 2^21 on) and, with both gradients, as much again
+// for the second set of planes.  Per logit that is 4 B written and read, then 4 B
+// written and read for each product.  In every form the product's epilogue reduces
+// each row of a tile to its maximum, sum of exponentials and target logit; the loss
+// alone stores no logits.
 //
 // The loss of a few rows (a token being scored) reads the weight once as it is, with
 // f32 multiply-adds: nothing is split, and that one read is what bounds it.
@@ -73,32 +78,40 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   if (!counted) xent_count(tgt, tdt, n, V, count);
   // Pieces of whole 256-row tiles, of even size; of 64 rows (the products' step in K)
   // where 256 do not fit the bound.
-  const bool in_place = xent_rows_in_place(ld);
-  const int64_t fit = (int64_t)(kPieceBytes / ((size_t)ld * (in_place ? 4 : 8)));
+  const int64_t fit = (int64_t)(kPieceBytes / ((size_t)ld * 4));
   const int64_t unit = fit >= 256 ? 256 : 64, most = std::max(unit, fit / unit * unit);
   const int64_t pieces = (n + most - 1) / most;
   const int64_t piece = ((n + pieces - 1) / pieces + unit - 1) / unit * unit;
-  float* logits = static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
-  float* planes = in_place ? logits : static_cast<float*>(scratch_alloc((size_t)std::min(piece, n) * ld * 4));
-  const __half* hi = reinterpret_cast<const __half*>(planes);
-  constexpr float inv = 1.0f / (1 << kF16Exp);
+  const size_t rows = (size_t)std::min(piece, n), row_bytes = (size_t)ld * 4;
+  float* logits = static_cast<float*>(scratch_alloc(rows * row_bytes));
+  __half* over = reinterpret_cast<__half*>(logits);   // planes in place of the logits
+  __half* entry = dw ? over : nullptr;
+  __half* even = dx && dw ? static_cast<__half*>(scratch_alloc(rows * row_bytes)) : dx ? over : nullptr;
+  // the scales of `entry`, and the rows' statistics
+  const int parts = f16_lse_parts((int)V);
+  const int64_t inv_pitch = f16_scales(ld), inv_rows = ((int64_t)rows + kF16Block - 1) / kF16Block;
+  float* inv = static_cast<float*>(scratch_alloc((size_t)(inv_rows * inv_pitch) * 4 + rows * ((size_t)parts * 8 + 4)));
+  float2* part = reinterpret_cast<float2*>(inv + inv_rows * inv_pitch);
+  float* at = reinterpret_cast<float*>(part + rows * parts);
   for (int64_t r0 = 0; r0 < n; r0 += piece) {
     const int64_t m = std::min(piece, n - r0);
+    const void* t = static_cast<const char*>(tgt) + r0 * (int64_t)dtype_size(tdt);
     F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), logits, ld, false, nullptr};
-    gemm_f16(g);
-    xent_rows(logits, planes, ld, m, V, tgt, tdt, r0, nll);
+    gemm_f16_lse(g, part, at, t, tdt);
+    xent_planes(logits, ld, m, V, {part, parts, at, t, tdt}, nll + r0, even, entry, inv, inv_pitch);
     if (dx) {
-      const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, false, 0, nullptr, inv};
+      const F16Operand dl{even, even + 64, m, ld, 2 * ld, false, 0, nullptr, 1.0f / (1 << kF16Exp), true};
       gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, count});
     }
     if (dw) {
-      const F16Operand dl{hi, hi + ld, m, ld, 2 * ld, true, 0, nullptr, inv};
+      const F16Operand dl{entry, entry + 64, m, ld, 2 * ld, true, 0, nullptr, 1.0f, true, inv, inv_pitch};
       const F16Operand xt = xc.kmajor(0, D, r0);
       if (tied) gemm_f16({(int)V, (int)D, (int)m, dl, xt, dw, D, r0 > 0, count});
       else gemm_f16({(int)D, (int)V, (int)m, xt, dl, dw, V, r0 > 0, count});
     }
   }
-  if (!in_place) scratch_free(planes);
+  scratch_free(inv);
+  if (even != over) scratch_free(even);
   scratch_free(logits);
   loss_mean(nll, n, count, loss);
   scratch_free(count);
@@ -120,7 +133,7 @@ void loss_only(const float* x, const float* w, const void* tgt, int tdt, bool ti
     const void* t = static_cast<const char*>(tgt) + r0 * (int64_t)dtype_size(tdt);
     F16Gemm g{(int)m, (int)V, (int)D, xr.kmajor(r0, m), wv.kmajor(0, V), nullptr, 0, false, nullptr};
     gemm_f16_lse(g, part, at, t, tdt);
-    xent_join(part, parts, at, t, tdt, V, m, nll + r0);
+    xent_join({part, parts, at, t, tdt}, V, m, nll + r0, nullptr);
   }
   scratch_free(part);
   loss_mean_counted(nll, n, tgt, tdt, V, loss);

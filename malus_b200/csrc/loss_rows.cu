@@ -108,75 +108,54 @@ __device__ __forceinline__ float join_factor(float m, float M, float c) {
   return m == -INFINITY ? 1.0f : tc::exp2_hw((m - M) * c);
 }
 
-// Four elements of a row's gradient, magnitudes at most 1, as the half planes that
-// the head's products read: hi in the first half of the row's memory, lo in the
-// second.
-__device__ __forceinline__ void store_planes(float* row, int ld, int e, float4 q) {
-  constexpr float up = (float)(1 << kF16Exp);
-  const float x[4] = {q.x * up, q.y * up, q.z * up, q.w * up};
-  __align__(8) __half h[4], l[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    h[j] = __float2half_rn(x[j]);
-    l[j] = __float2half_rn(x[j] - __half2float(h[j]));
-  }
-  __half* p = reinterpret_cast<__half*>(row);
-  *reinterpret_cast<uint2*>(p + e) = *reinterpret_cast<uint2*>(h);
-  *reinterpret_cast<uint2*>(p + ld + e) = *reinterpret_cast<uint2*>(l);
-}
-// Four probabilities from column e on, less 1 at the target.
-__device__ __forceinline__ float4 less_hot(float4 q, int t, int e) {
+// Four probabilities (times `one`) from column e on, less 1 at the target.
+__device__ __forceinline__ float4 less_hot(float4 q, int t, int e, float one = 1.0f) {
   const unsigned o = (unsigned)(t - e);
   if (o < 4) {
-    if (o == 0) q.x -= 1.0f;
-    if (o == 1) q.y -= 1.0f;
-    if (o == 2) q.z -= 1.0f;
-    if (o == 3) q.w -= 1.0f;
+    if (o == 0) q.x -= one;
+    if (o == 1) q.y -= one;
+    if (o == 2) q.z -= one;
+    if (o == 3) q.w -= one;
   }
   return q;
 }
 
-// PLANES: the gradient as half planes, else as f32 (in place).
-template <bool PLANES>
+// The cross entropy's rows; the gradient in place.
 struct XentRows {
-  const float* logits;
-  float* out;          // the gradient: over the logits, or memory of its own (null: none)
+  float* logits;
+  bool grad;           // whether the gradient is wanted
   int ld, V_;
   int64_t rows;
   const void* tgt;
   int tdt;
-  int64_t row0;
   float* nll;
-  int* count;          // counts the rows (null: someone else does)
+  int* count;          // counts the rows
   int32_t* err;
   __device__ __forceinline__ const float* row(int64_t r) const { return logits + r * ld; }
   __device__ __forceinline__ int width() const { return ld; }   // groups cover the pitch
   __device__ __forceinline__ int V() const { return V_; }       // logits among them
   // four elements of a row's gradient
   __device__ __forceinline__ void store(float* row_out, int e, float4 q) const {
-    if (PLANES) store_planes(row_out, ld, e, q);
-    else *reinterpret_cast<float4*>(row_out + e) = q;
+    *reinterpret_cast<float4*>(row_out + e) = q;
   }
   // a row's value, by one thread
   __device__ __forceinline__ void tell(int64_t r, int64_t t, bool counted, float v) const {
-    nll[row0 + r] = v;
-    if (!count) return;
+    nll[r] = v;
     if (counted) atomicAdd(count, 1);   // whole numbers: the order does not matter
     else if (t >= V_) atomicExch(err, kErrId);
   }
 };
 
-template <int NV, class Op>
-__global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const Op d) {
+template <int NV>
+__global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d) {
   const int lane = threadIdx.x & 31, ld = d.ld, V = d.V_;
   for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < d.rows; r += (int64_t)gridDim.x * kWarps) {
-    const float* row = d.row(r);
-    float* out = d.out + r * ld;
-    const int64_t t = id_at(d.tgt, d.tdt, d.row0 + r);
+    float* row = d.logits + r * ld;
+    const int64_t t = id_at(d.tgt, d.tdt, r);
     if (t < 0 || t >= V) {
       if (lane == 0) d.tell(r, t, false, 0.0f);
-      if (!d.out) continue;
-      for (int g = lane; g < ld / 4; g += 32) d.store(out, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (!d.grad) continue;
+      for (int g = lane; g < ld / 4; g += 32) d.store(row, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
       continue;
     }
     const float zt = row[t];
@@ -188,13 +167,13 @@ __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const Op d) {
     }
     const RowStat st = warp_stat(v, kLog2e);   // the whole row is in registers after it
     if (lane == 0) d.tell(r, t, true, logf(st.sum) - (zt - st.max));
-    if (!d.out) continue;
+    if (!d.grad) continue;
     const float f = 1.0f / st.sum;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int e = 4 * (k * 32 + lane);
       if (e < ld)   // columns from V on hold exp(-inf) = 0
-        d.store(out, e, less_hot(make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f), (int)t, e));
+        d.store(row, e, less_hot(make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f), (int)t, e));
     }
   }
 }
@@ -283,28 +262,144 @@ __global__ void __launch_bounds__(1024) k_loss_mean(float* __restrict__ v, const
   }
 }
 
-// nll of a row from its parts' (maximum, sum of exponentials) and its target's
-// logit; a warp per row
-__global__ void __launch_bounds__(256) k_xent_join(const float2* __restrict__ part, int parts,
-                                                   const float* __restrict__ at, const void* __restrict__ tgt, int tdt,
-                                                   int64_t V, int64_t n, float* __restrict__ nll) {
-  const int lane = threadIdx.x & 31;
+// nll of row r from its parts' (maximum, sum of exponentials) and its target's logit,
+// and what its gradient takes, by W threads (a warp, or one)
+template <int W>
+__device__ __forceinline__ XentStat join_row(const XentParts& p, int64_t V, int64_t r) {
+  const int lane = W == 32 ? threadIdx.x & 31 : 0;
+  const int64_t t = id_at(p.tgt, p.tdt, r);
+  if (t < 0 || t >= V) return {0.0f, 0.0f, -1, 0.0f};
+  const float2* part = p.part + r * p.parts;
+  float M = -INFINITY, s = 0.0f;
+  for (int i = lane; i < p.parts; i += W) M = fmaxf(M, part[i].x);
+  if (W == 32) M = wmax(M);
+  for (int i = lane; i < p.parts; i += W) {
+    const float2 o = part[i];
+    s += o.y * (o.x == -INFINITY ? 1.0f : exp2f((o.x - M) * kLog2e));   // -inf only: the sum is 0 or NaN
+  }
+  if (W == 32) s = wsum(s);
+  return {M == -INFINITY ? 0.0f : M, 1.0f / s, (int)t, logf(s) - (p.at[r] - M)};
+}
+__global__ void __launch_bounds__(256) k_xent_join(const XentParts p, int64_t V, int64_t n, float* __restrict__ nll,
+                                                   XentStat* __restrict__ stat) {
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += (int64_t)gridDim.x * 8) {
-    const int64_t t = id_at(tgt, tdt, r);
-    if (t < 0 || t >= V) {
-      if (lane == 0) nll[r] = 0.0f;
+    const XentStat s = join_row<32>(p, V, r);
+    if ((threadIdx.x & 31) == 0) {
+      nll[r] = s.nll;
+      if (stat) stat[r] = s;
+    }
+  }
+}
+
+// A tile of kF16Block rows and 64 columns of f32 logits to the half planes of dl =
+// softmax - onehot, in the grouped layout of F16Operand, in one pass: 4 B read per
+// logit and 4 B written per set of planes (2048 x 50304, both sets: 197 us, 6.3 TB/s; with
+// 256 threads of 16 groups each 265 us).  EVEN: at one scale,
+// 2^kF16Exp, for a product that sums over the vocabulary, where the largest of a
+// token's gradients sets the accuracy.  ENTRY: scaled per vocabulary entry by the
+// largest of its column in the tile, for the product that sums over the tokens:
+// there each entry's row of dweight has a size of its own, from 1 down to the
+// smallest floats.  One of the sets may lie over the logits: a tile's planes cover
+// just the bytes of its logits.  Columns from V on are zeros, and rows left out.
+// Rows of few parts (stat null) are joined here, by every tile of theirs, and the
+// first one writes their nll.
+constexpr int kTileThreads = 512;
+static_assert(kTileThreads >= kF16Block, "a thread per row");
+
+// Two scaled values as halves, hi and what is left.
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t* h, uint32_t* l) {
+  const __half2 hi = __floats2half2_rn(x, y);
+  const float2 b = __half22float2(hi);
+  const __half2 lo = __floats2half2_rn(x - b.x, y - b.y);
+  *h = *reinterpret_cast<const uint32_t*>(&hi);
+  *l = *reinterpret_cast<const uint32_t*>(&lo);
+}
+__device__ __forceinline__ void store_split(__half* p, float4 v) {
+  uint2 h, l;
+  split_pair(v.x, v.y, &h.x, &l.x);
+  split_pair(v.z, v.w, &h.y, &l.y);
+  *reinterpret_cast<uint2*>(p) = h;
+  *reinterpret_cast<uint2*>(p + 64) = l;
+}
+
+template <bool EVEN, bool ENTRY>
+__global__ void __launch_bounds__(kTileThreads, 1024 / kTileThreads)
+k_xent_planes(const float* logits, int64_t ld, int64_t n, int64_t V, const XentStat* __restrict__ stat, const XentParts p,
+              float* __restrict__ nll, __half* even, __half* entry, float* __restrict__ inv, int64_t inv_pitch) {
+  constexpr int kStep = kTileThreads / 16, kRows = kF16Block / kStep, kTileWarps = kTileThreads / 32;
+  constexpr float one = (float)(1 << kF16Exp);
+  __shared__ XentStat st[kF16Block];
+  __shared__ __align__(16) float sh[kTileWarps][64], ups[64];
+  const int groups = (int)(ld / 64), g = (int)(blockIdx.x % groups), tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t block = blockIdx.x / groups, r0 = block * kF16Block;
+  const int c = g * 64 + 4 * tx, rows = (int)min((int64_t)kF16Block, n - r0);
+  float4 q[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = ty + kStep * i;
+    q[i] = r < rows ? *reinterpret_cast<const float4*>(logits + (r0 + r) * ld + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  if (threadIdx.x < kF16Block) {
+    const int64_t r = r0 + threadIdx.x;
+    XentStat s = {0.0f, 0.0f, -1, 0.0f};
+    if (threadIdx.x < rows) {
+      s = stat ? stat[r] : join_row<1>(p, V, r);
+      if (!stat && g == 0) nll[r] = s.nll;
+    }
+    st[threadIdx.x] = s;
+  }
+  __syncthreads();
+  float cm[4] = {};
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const XentStat s = st[ty + kStep * i];
+    if (s.target < 0) {
+      q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       continue;
     }
-    float M = -INFINITY;
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, part[r * parts + i].x);
-    M = wmax(M);
-    float s = 0.0f;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 o = part[r * parts + i];
-      s += o.y * (o.x == -INFINITY ? 1.0f : exp2f((o.x - M) * kLog2e));   // -inf only: the sum is 0 or NaN
+    const float f = s.inv_sum * one;   // dl times 2^kF16Exp
+    q[i].x = tc::exp2_hw((q[i].x - s.max) * kLog2e) * f;
+    q[i].y = tc::exp2_hw((q[i].y - s.max) * kLog2e) * f;
+    q[i].z = tc::exp2_hw((q[i].z - s.max) * kLog2e) * f;
+    q[i].w = tc::exp2_hw((q[i].w - s.max) * kLog2e) * f;
+    if (c + 4 > V) {
+      if (c >= V) q[i].x = 0.0f;
+      if (c + 1 >= V) q[i].y = 0.0f;
+      if (c + 2 >= V) q[i].z = 0.0f;
+      q[i].w = 0.0f;
     }
-    s = wsum(s);
-    if (lane == 0) nll[r] = logf(s) - (at[r] - M);
+    q[i] = less_hot(q[i], s.target, c, one);
+    if (ENTRY) {   // a NaN passes by: its row makes all of dweight NaN
+      cm[0] = fmaxf(cm[0], fabsf(q[i].x));
+      cm[1] = fmaxf(cm[1], fabsf(q[i].y));
+      cm[2] = fmaxf(cm[2], fabsf(q[i].z));
+      cm[3] = fmaxf(cm[3], fabsf(q[i].w));
+    }
+  }
+  float4 up = make_float4(one, one, one, one);
+  if (ENTRY) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cm[j] = fmaxf(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], 16));
+    if ((threadIdx.x & 16) == 0)
+      *reinterpret_cast<float4*>(&sh[threadIdx.x >> 5][4 * tx]) = make_float4(cm[0], cm[1], cm[2], cm[3]);
+    __syncthreads();
+    if (threadIdx.x < 64) {   // a column's scale
+      float m = 0.0f, u, iv;
+      for (int k = 0; k < kTileWarps; ++k) m = fmaxf(m, sh[k][threadIdx.x]);
+      f16_scale(__float_as_uint(m), &u, &iv);
+      ups[threadIdx.x] = u;
+      inv[block * inv_pitch + g * 64 + threadIdx.x] = iv * (1.0f / one);
+    }
+    __syncthreads();
+    up = *reinterpret_cast<const float4*>(ups + 4 * tx);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = ty + kStep * i;
+    if (r >= rows) break;
+    const int64_t at = (r0 + r) * 2 * ld + g * 128 + 4 * tx;
+    if (EVEN) store_split(even + at, q[i]);
+    if (ENTRY) store_split(entry + at, make_float4(q[i].x * up.x, q[i].y * up.y, q[i].z * up.z, q[i].w * up.w));
   }
 }
 
@@ -628,34 +723,33 @@ __device__ __forceinline__ void ring_map(R_& R, RowStat st, float c, F&& f) {
   }
 }
 
-template <class R_, bool PLANES>
-__device__ __forceinline__ void ring_rows(R_& R, const XentRows<PLANES>& d, float2* table, int64_t first, int64_t step) {
+template <class R_>
+__device__ __forceinline__ void ring_rows(R_& R, const XentRows& d, float2* table, int64_t first, int64_t step) {
   const int tid = (int)threadIdx.x, nt = R.chunk / 2;
-  int64_t next = first < d.rows ? id_at(d.tgt, d.tdt, d.row0 + first) : -1;
+  int64_t next = first < d.rows ? id_at(d.tgt, d.tdt, first) : -1;
   uint32_t turn = 0;
   for (int64_t r = first; r < d.rows; r += step, ++turn, R.row_done()) {
-    const float* row = d.row(r);
-    float* out = d.out + r * d.ld;
+    float* row = d.logits + r * d.ld;
     const int64_t t = next;
-    if (r + step < d.rows) next = id_at(d.tgt, d.tdt, d.row0 + r + step);
+    if (r + step < d.rows) next = id_at(d.tgt, d.tdt, r + step);
     if (t < 0 || t >= d.V_) {
       if (tid == 0) d.tell(r, t, false, 0.0f);
       ring_skip(R, R_::STAY ? 1 : 2);   // the copies have left the row before it is written
       ring_barrier(R);
-      if (d.out)
-        for (int g = tid; g < R.groups; g += nt) d.store(out, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (d.grad)
+        for (int g = tid; g < R.groups; g += nt) d.store(row, 4 * g, make_float4(0.f, 0.f, 0.f, 0.f));
       continue;
     }
     const float zt = tid == 0 ? row[t] : 0.0f;
-    const RowStat st = ring_stat(R, kLog2e, table, turn, !d.out);   // its barrier: a row that stays has landed
+    const RowStat st = ring_stat(R, kLog2e, table, turn, !d.grad);   // its barrier: a row that stays has landed
     if (tid == 0) d.tell(r, t, true, logf(st.sum) - (zt - st.max));
-    if (!d.out) {
+    if (!d.grad) {
       if (!R_::STAY) ring_skip(R, 1);
       continue;
     }
     const float f = 1.0f / st.sum;
     ring_map(R, st, kLog2e, [&](int g, float4 e) {   // columns from V on hold exp(-inf) = 0
-      d.store(out, 4 * g, less_hot(make_float4(e.x * f, e.y * f, e.z * f, e.w * f), (int)t, 4 * g));
+      d.store(row, 4 * g, less_hot(make_float4(e.x * f, e.y * f, e.z * f, e.w * f), (int)t, 4 * g));
     });
   }
 }
@@ -793,22 +887,11 @@ void with_warp_rows(int64_t groups, int64_t rows, F&& f) {
   else if (nv <= 4) f.template operator()<4>(blocks);
   else f.template operator()<kNV>(blocks);
 }
-template <bool PLANES>
 struct XentShort {
-  const XentRows<PLANES>& d;
+  const XentRows& d;
   template <int NV>
   void operator()(unsigned blocks) const { k_xent_rows_warp<NV><<<blocks, 32 * kWarps, 0, stream()>>>(d); }
 };
-template <bool PLANES>
-void run_xent(const XentRows<PLANES>& d) {
-  if (d.rows == 0) return;
-  const int pid = prof_begin_named("k_xent_rows", (d.out ? 8.0 : 4.0) * (double)d.rows * (double)d.ld);
-  if (d.ld <= kShort) with_warp_rows(d.ld / 4, d.rows, XentShort<PLANES>{d});
-  else launch_ring(d, d.ld / 4);
-  count_launch();
-  after_launch("k_xent_rows");
-  prof_end(pid);
-}
 struct DistillShort {
   const Distill& d;
   template <int NV>
@@ -823,24 +906,45 @@ void xent_count(const void* targets, int tgt_dtype, int64_t n, int64_t V, int* c
   after_launch("k_xent_count");
 }
 
-bool xent_rows_in_place(int64_t ld) { return ld / 4 <= kRingGroups; }
-
-void xent_rows(const float* logits, float* planes, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype,
-               int64_t row0, float* nll) {
-  run_xent(XentRows<true>{logits, planes, (int)ld, (int)V, n, targets, tgt_dtype, row0, nll, nullptr,
-                          device_error_word()});
+void xent_planes(const float* logits, int64_t ld, int64_t n, int64_t V, const XentParts& p, float* nll, __half* even,
+                 __half* entry, float* inv, int64_t inv_pitch) {
+  const int64_t blocks = (n + kF16Block - 1) / kF16Block * (ld / 64);
+  if (blocks > INT32_MAX) panic("xent_planes: %lld tiles", (long long)blocks);
+  // up to 1024 entries a tile's threads join their rows themselves (training 16384 x 384
+  // x 65: 130 us, 136 with a launch for it)
+  XentStat* stat = nullptr;
+  if (p.parts > 8) {
+    stat = static_cast<XentStat*>(scratch_alloc((size_t)n * sizeof(XentStat)));
+    xent_join(p, V, n, nll, stat);
+  }
+  const int pid = prof_begin_named("k_xent_planes", (even && entry ? 12.0 : 8.0) * (double)n * (double)ld);
+  auto go = [&](auto kernel) {
+    kernel<<<(unsigned)blocks, kTileThreads, 0, stream()>>>(logits, ld, n, V, stat, p, nll, even, entry, inv, inv_pitch);
+  };
+  if (even && entry) go(k_xent_planes<true, true>);
+  else if (even) go(k_xent_planes<true, false>);
+  else go(k_xent_planes<false, true>);
+  count_launch();
+  after_launch("k_xent_planes");
+  prof_end(pid);
+  scratch_free(stat);
 }
 
 void xent_rows_f32(float* logits, int64_t ld, int64_t n, int64_t V, const void* targets, int tgt_dtype, float* nll,
                    int* count, bool grad) {
-  run_xent(XentRows<false>{logits, grad ? logits : nullptr, (int)ld, (int)V, n, targets, tgt_dtype, 0, nll, count,
-                           device_error_word()});
+  if (n == 0) return;
+  const XentRows d{logits, grad, (int)ld, (int)V, n, targets, tgt_dtype, nll, count, device_error_word()};
+  const int pid = prof_begin_named("k_xent_rows", (grad ? 8.0 : 4.0) * (double)n * (double)ld);
+  if (ld <= kShort) with_warp_rows(ld / 4, n, XentShort{d});
+  else launch_ring(d, (int)(ld / 4));
+  count_launch();
+  after_launch("k_xent_rows");
+  prof_end(pid);
 }
 
-void xent_join(const float2* part, int parts, const float* at, const void* targets, int tgt_dtype, int64_t V, int64_t n,
-               float* nll) {
+void xent_join(const XentParts& p, int64_t V, int64_t n, float* nll, XentStat* stat) {
   if (n == 0) return;
-  k_xent_join<<<grid_for((size_t)n * 32, 256), 256, 0, stream()>>>(part, parts, at, targets, tgt_dtype, V, n, nll);
+  k_xent_join<<<grid_for((size_t)n * 32, 256), 256, 0, stream()>>>(p, V, n, nll, stat);
   count_launch();
   after_launch("k_xent_join");
 }

@@ -1,0 +1,57 @@
+"""GPU: the head's weight gradient of vocabulary entries that are hardly ever
+predicted, entry by entry.  Their softmax gradients are 1e-5 to 1e-20 in every
+token, and an optimiser that divides by a gradient's own size sees each row at
+full scale, so every row of dweight is held to its own magnitudes.
+
+Tolerances (u = 2^-24).  x and weight hold small multiples of 1/2: every product
+and sum of the logits is exact, so log q carries only the softmax's own error,
+(80 + 8 |z - max|) u as in the distillation tests, and dl = q - onehot that error
+of q and two roundings.  No absolute error is allowed for: the products' bound
+(prod_tol) is relative to the terms and to the largest one of the row."""
+import numpy as np
+import pytest
+
+from test_gpu_linear_xent import U, both_products, mode, prod_tol, run  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(n, D, V, seed):
+    r = np.random.default_rng(seed)
+    x = r.choice(np.array([-2, -1, 1, 2], np.float32), (n, D))
+    w = r.choice(np.array([-0.5, 0, 0.5], np.float32), (V, D))
+    x[:, 0] = 1.0
+    w[:, 0] = -np.floor(30.0 * np.arange(V) / V)   # the later an entry, the rarer
+    t = r.integers(0, max(1, V // 4), n).astype(np.int32)
+    t[r.random(n) < 0.2] = -1
+    return x, w, t
+
+
+def reference(x, w, t):
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    n = x.shape[0]
+    ok = t >= 0
+    cnt = max(1, int(ok.sum()))
+    z = x @ w.T
+    z -= z.max(1, keepdims=True)
+    lq = z - np.log(np.exp(z).sum(1, keepdims=True))
+    q = np.exp(lq) * ok[:, None]
+    dl = q.copy()
+    dl[np.arange(n)[ok], t[ok]] -= 1
+    edl = q * U * (80 + 8 * np.abs(z)) + 2 * U * np.abs(dl)
+    ad, ax = np.abs(dl), np.abs(x)
+    tw = (edl.T @ ax + prod_tol(ad.T, ax.T, n) + 8 * U * (ad.T @ ax)) / cnt
+    return dl.T @ x / cnt, tw
+
+
+@pytest.mark.parametrize("tied", [True, False])
+@pytest.mark.parametrize("n,D,V", [(700, 32, 4000), (257, 33, 1001), (20000, 32, 300), (300, 16, 70001), (64, 20, 90)])
+@both_products
+def test_rows_of_rare_entries(M, rt, mode, n, D, V, tied):  # noqa: F811
+    x, w, t = inputs(n, D, V, n + V)
+    want, tol = reference(x, w, t)
+    dw = run(M, x, w, t, tied)[3]
+    assert (np.abs(want).max(1) < 2.0 ** -38).any() or V < 1000   # entries below any fixed grid are among them
+    bad = ~(np.abs(dw - want) <= tol + 1e-36)
+    assert not bad.any(), f"{bad.any(1).sum()} of {V} rows off, worst {np.max(np.abs(dw - want) / (tol + 1e-36)):.3g}"
+    assert rt.malus_device_error() == 0
