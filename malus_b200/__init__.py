@@ -425,6 +425,27 @@ def distill(logits: Tensor, ids: Tensor, teacher: Tensor, temperature: float = 1
     return Tensor(loss), Tensor(kl[0]), Tensor(dl[0]) if grad else None
 
 
+def record_layernorm_affine(x: Tensor, weight: Tensor | None, bias: Tensor | None, y: Tensor, stats: Tensor) -> None:
+    """Tape record of y, stats = layernorm_affine(x, weight, bias).  The tape holds
+    references of its own: every Tensor stays the caller's to close or drop."""
+    lib = load()
+    lib.tensor_retain(stats.h)   # the record takes this reference over
+    lib.tape_record_layernorm_affine(x.h, _h(weight), _h(bias), y.h, stats.h)
+
+
+def record_loss(inputs, grads, loss: Tensor) -> None:
+    """Tape record of a loss that came with its gradients: grads[i] is its gradient
+    with respect to inputs[i], as linear_xent (x, weight: dx, dweight) and distill
+    (logits: dlogits) return them.  References as in record_layernorm_affine."""
+    lib = load()
+    n = len(inputs)
+    if len(grads) != n or any(g is None for g in grads):
+        raise ValueError(f"record_loss needs a gradient for each of its {n} inputs")
+    for g in grads:
+        lib.tensor_retain(g.h)   # the record takes these references over
+    lib.tape_record_loss((C.c_int64 * n)(*(t.h for t in inputs)), (C.c_int64 * n)(*(g.h for g in grads)), n, loss.h)
+
+
 class GPT:
     """The compiled nanoGPT training step (malus_gpt_*)."""
 
