@@ -718,15 +718,15 @@ CUtensorMap map_of(const F16Operand& o, const __half* plane) {
 
 template <int MODE>
 cudaLaunchConfig_t config(int grid, cudaLaunchAttribute* at) {
-  static bool attr = false;
-  if (!attr) {
+  static const bool ready = [] {   // once, whichever thread comes first
     MALUS_CUDA(cudaFuncSetAttribute(k_gemm_f16<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     // the register split draws on what the launch reserves: fewer would wait forever
     cudaFuncAttributes fa;
     MALUS_CUDA(cudaFuncGetAttributes(&fa, k_gemm_f16<MODE>));
     if (fa.numRegs < kRegsLaunch) panic("gemm_f16: %d registers per thread at launch, %d needed", fa.numRegs, kRegsLaunch);
-    attr = true;
-  }
+    return true;
+  }();
+  (void)ready;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kThreads);

@@ -362,7 +362,8 @@ void few(const float* x, const float* w, const void* tgt, int tdt, bool tied, in
   float* at = reinterpret_cast<float*>(part + (int64_t)n * grid);
   const int pid = prof_begin_named("k_head_few", 4.0 * (double)V * D);
   auto go = [&](auto kernel, size_t smem) {
-    MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the limit is the function's, for every thread's calls: always the same one
+    MALUS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     kernel<<<grid, 32 * kFewWarps, smem, stream()>>>(x, w, n, D, V, tgt, tdt, part, at);
   };
   const size_t rows = (size_t)N * ((D + 127) / 128 * 128) * 4;

@@ -1002,8 +1002,8 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   if (n) {
     const Distill d{x, ent, flag, count, n, V, (int)K, temperature, part, hd ? fptr(hd) : nullptr, parts,
                     device_error_word()};
-    if (K > 512)   // over 48 KB
-      MALUS_CUDA(cudaFuncSetAttribute(k_teacher, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K * 64));
+    if (K > 512)   // past the default limit from 768 on; the same limit for every thread's calls
+      MALUS_CUDA(cudaFuncSetAttribute(k_teacher, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxEntries * 64));
     k_teacher<<<grid_for((size_t)n * 32, 256), 256, (size_t)K * 64, stream()>>>(
         idp, idt, te, n, (int)K, V, kLog2e / temperature, ent, flag, count, device_error_word());
     const int pid = prof_begin_named("k_distill_rows", (hd ? 8.0 : 4.0) * (double)n * (double)V);
