@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_xent_rows_warp(const XentRows d
       v[k] = e + 4 <= V ? *reinterpret_cast<const float4*>(row + e) : load_edge(row, V, e);
     }
     const RowStat st = warp_stat(v, kLog2e);   // the whole row is in registers after it
+    __syncwarp();   // shuffles order no memory: every lane has read the row before one writes over it
     if (lane == 0) d.tell(r, t, true, logf(st.sum) - (zt - st.max));
     if (!d.grad) continue;
     const float f = 1.0f / st.sum;
