@@ -633,6 +633,9 @@ __device__ __forceinline__ void ring_feed(R_& R, const Op& op, int64_t first, in
       const int slot = R.at(j);
       if (R.round && !R.dead) R.dead = !wait_for(R.empty_of(slot), (R.round - 1) & 1, R.err, 53);
       if (R.dead) break;
+      // what this slot held was written by element at its row's ends, and read, before
+      // the copy may land on it
+      tc::fence_async_smem();
       const int lo = (j < R.chunks ? j : j - R.chunks) * R.chunk, hi = min(lo + R.chunk, R.groups);
       float4* at = R.buf + slot * R.chunk - lo;
       if (lane == 0 && lo == 0 && s.w0) at[0] = head;
