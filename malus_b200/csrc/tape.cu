@@ -255,6 +255,8 @@ void tape_record_layernorm_affine(int64_t x, int64_t weight, int64_t bias, int64
     tensor_release(stats);
     return;
   }
+  if (!stats) panic("tape_record_layernorm_affine needs the forward pass's stats");
+  if (!same_shape(x, out)) panic("tape_record_layernorm_affine: the output has not x's shape");
   for (int64_t h : {x, weight, bias, out}) tensor_retain(h);
   t_tape.nodes.push_back(Node{kLayernormAffine, {x, weight, bias, stats}, out, {}});
 }
