@@ -293,10 +293,10 @@ void malus_layernorm_affine_bwd(int64_t x, int64_t weight, int64_t stats, int64_
  * V is limited to 2^24. */
 int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
                           int64_t* dweight);
-/* Which products malus_linear_xent uses: -1 (default) the measured rule (f32
- * multiply-adds for small problems and few rows, half planes on the tensor cores
- * otherwise), 0 half planes always, 1 multiply-adds always (up to 16384 rows).
- * Returns the previous setting.  A tuning and test hook. */
+/* Which products malus_linear_xent uses in the calling thread: -1 (default) the
+ * measured rule (f32 multiply-adds for small problems and few rows, half planes on
+ * the tensor cores otherwise), 0 half planes always, 1 multiply-adds always (up to
+ * 16384 rows).  Returns the thread's previous setting.  A tuning and test hook. */
 int32_t malus_linear_xent_mode(int32_t mode);
 /* Distillation from a teacher's top logits: logits [N, V], and per row K <= 1024
  * entries ids [N, K] with teacher logits [N, K].  p = softmax over the row's

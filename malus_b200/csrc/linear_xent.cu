@@ -27,6 +27,8 @@
 #include "linear_xent.cuh"
 #include "loss_rows.cuh"
 
+#include <utility>
+
 namespace malus {
 namespace {
 
@@ -377,11 +379,11 @@ void few(const float* x, const float* w, const void* tgt, int tdt, bool tied, in
   scratch_free(part);
 }
 
-std::atomic<int> g_mode{-1};
+thread_local int t_mode = -1;   // one thread's choice leaves the others' results alone
 
 // Rows that take this path: x in shared memory beside the block's sums.
 bool few_rows(int64_t n, int64_t D) {
-  if (n < 1 || n > kFewRows || g_mode.load(std::memory_order_relaxed) != -1) return false;
+  if (n < 1 || n > kFewRows || t_mode != -1) return false;
   const int64_t N = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
   return N * (D + 127 + kFewWarps * 128) * 4 <= kFewSmem;
 }
@@ -395,7 +397,7 @@ extern "C" {
 
 int32_t malus_linear_xent_mode(int32_t mode) {
   if (mode < -1 || mode > 1) panic("malus_linear_xent_mode(%d): -1, 0 or 1", mode);
-  return g_mode.exchange(mode);
+  return std::exchange(t_mode, (int)mode);
 }
 
 int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
@@ -430,8 +432,7 @@ int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t ti
     if (dweight) *dweight = 0;
     return loss;
   }
-  const int mode = g_mode.load(std::memory_order_relaxed);
-  if (n && (mode < 0 ? head_small((int64_t)n, (int64_t)D, (int64_t)V, hx || hw) : mode == 1 && n <= 16384)) {
+  if (n && (t_mode < 0 ? head_small((int64_t)n, (int64_t)D, (int64_t)V, hx || hw) : t_mode == 1 && n <= 16384)) {
     head_small_run(xp, wp, tp, tdt, tied != 0, (int64_t)n, (int64_t)D, (int64_t)V, fptr(hn), fptr(loss),
                    hx ? fptr(hx) : nullptr, hw ? fptr(hw) : nullptr);
     if (nll) *nll = hn;
