@@ -159,13 +159,21 @@ void malus_tape_registry_lens(int64_t* leaves, int64_t* grads);
 void* malus_tensor_data(int64_t h);
 int32_t malus_tensor_dtype(int64_t h);
 /* All of the above in one call: out = (data pointer, dtype, rank, shape...), 11
- * words at most; returns the rank. */
+ * words at most; returns the rank.  From then on the memory is shared, as
+ * malus_tensor_wrap_shared says. */
 int32_t malus_tensor_describe(int64_t h, int64_t* out);
 /* Copy a tensor to / from host memory (synchronous). */
 void malus_tensor_read(int64_t h, void* dst, size_t bytes);
 void malus_tensor_write(int64_t h, const void* src, size_t bytes);
-/* Wrap caller-owned device memory as a handle (not pooled; never freed). */
+/* Wrap caller-owned device memory as a handle (not pooled; never freed).  GEMMs may
+ * keep operand planes of it and products of it may be deferred: what writes it
+ * must be the runtime. */
 int64_t malus_tensor_wrap(int32_t dtype, void* dev_ptr, const size_t* shape, size_t ndims);
+/* The same for memory that another library may rewrite between calls: nothing
+ * derived from it is kept from one call for the next, and no result of it is
+ * deferred.  Views of it (permutes, reshapes), the tape's records and captured graphs
+ * read it when they are used. */
+int64_t malus_tensor_wrap_shared(int32_t dtype, void* dev_ptr, const size_t* shape, size_t ndims);
 /* Reset the Philox call counter (metal.rs:1713-1715 is thread-local; the
  * reference resets it only per thread start). */
 void malus_rng_reset(uint64_t counter);

@@ -121,6 +121,7 @@ SIGNATURES: dict[str, tuple] = {
     "malus_tensor_read": (None, [i64, vp, sz]),
     "malus_tensor_write": (None, [i64, vp, sz]),
     "malus_tensor_wrap": (i64, [i32, vp, P_sz, sz]),
+    "malus_tensor_wrap_shared": (i64, [i32, vp, P_sz, sz]),
     "malus_rng_reset": (None, [u64]),
     "malus_philox4x32_10": (None, [C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "malus_set_device": (None, [i32]),
@@ -290,18 +291,21 @@ class Tensor:
     @staticmethod
     def wrap(ptr: int, shape, dtype=np.float32) -> "Tensor":
         """A handle for caller-owned device memory: contiguous row-major data
-        of `shape` at the device address `ptr`, which must stay alive as long as
-        the handle and, since all work runs on the runtime's own stream
-        (malus_stream), until the work queued on it is done.  Work that another
-        stream still has to do on the memory is the caller's to wait for."""
+        of `shape` at the device address `ptr`.  It may be rewritten between calls,
+        and must stay alive as long as the handle, views of it (permutes, reshapes),
+        tape records and captured graphs that hold it and, since all work runs on the
+        runtime's own stream (malus_stream), until the work queued on it is done.
+        Work that another stream still has to do on the memory is the caller's to
+        wait for."""
         s, n = _shape_arr(shape)
-        return Tensor(load().malus_tensor_wrap(_DTYPE_OF[dtype], ptr, s, n))
+        return Tensor(load().malus_tensor_wrap_shared(_DTYPE_OF[dtype], ptr, s, n))
 
     @property
     def __cuda_array_interface__(self) -> dict:
         """The data for another library on the same GPU, without a copy.  It is
         written on the runtime's stream: wait for that (gpu_barrier) before
-        reading it on another, and keep this object alive meanwhile."""
+        reading it on another, and keep this object alive meanwhile.  Writes to it
+        are seen by the calls that follow them (wait for the writing stream first)."""
         d = _DESCRIBE()
         n = load().malus_tensor_describe(self.h, d)
         shape = tuple(d[3:3 + n])

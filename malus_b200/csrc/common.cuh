@@ -41,6 +41,7 @@ struct Storage {
   int aliases;       // number of TensorBuffers sharing this storage
   bool owned;        // false for malus_tensor_wrap'd memory
   uint64_t id;       // unique per storage for the process (never reused)
+  bool shared = false;   // another library writes it too: nothing derived from it is kept or put off
 };
 
 // One logical dimension of a strided view: index i lies at element offset

@@ -115,13 +115,18 @@ int64_t sum_to_shape(int64_t g, const Shape& target) {
 // save matters) whose consumers can read them fused.
 constexpr size_t kLazyMin = (size_t)1 << 16;
 
+// Memory that another library may rewrite between two calls.
+bool is_shared(int64_t h) { return tb(h)->st && tb(h)->st->shared; }
+
 bool one_element_f32(int64_t h) { return tb(h)->len == 1 && tb(h)->dtype == MALUS_F32; }
 
 // a * b for a one-element b, deferred (the result has a's shape when b's rank
 // does not exceed a's); 0 when not applicable.
 int64_t lazy_scale(int64_t a, int64_t b) {
   auto *ta = tb(a), *tb_ = tb(b);
-  if (ta->dtype != MALUS_F32 || ta->len < kLazyMin || !one_element_f32(b) || tb_->ndim > ta->ndim) return 0;
+  if (ta->dtype != MALUS_F32 || ta->len < kLazyMin || !one_element_f32(b) || tb_->ndim > ta->ndim || is_shared(a) ||
+      is_shared(b))
+    return 0;
   int64_t z = make_lazy(ta->shape, ta->ndim, a, b, 0);
   tb(z)->causal_zero = ta->causal_zero;   // 0 * s stays 0 (the multiplier is taken to be finite)
   return z;
@@ -132,7 +137,7 @@ int64_t lazy_scale(int64_t a, int64_t b) {
 int64_t lazy_colscale(int64_t a, int64_t b) {
   auto *ta = tb(a), *tw = tb(b);
   if (ta->dtype != MALUS_F32 || ta->len < kLazyMin || ta->lazy || ta->ndim < 1 || tw->dtype != MALUS_F32 ||
-      tw->ndim != 1 || tw->len < 2 || tw->len != ta->shape[ta->ndim - 1])
+      tw->ndim != 1 || tw->len < 2 || tw->len != ta->shape[ta->ndim - 1] || is_shared(a) || is_shared(b))
     return 0;
   return make_lazy(ta->shape, ta->ndim, a, 0, 0, b);
 }
@@ -143,7 +148,7 @@ int64_t lazy_add(int64_t a, int64_t b) {
   auto *ta = tb(a), *tm = tb(b);
   if (!ta->lazy || !ta->lazy->scale || ta->lazy->addend || ta->lazy->colscale || tm->dtype != MALUS_F32 ||
       tm->ndim > ta->ndim ||
-      tm->len == 0)
+      tm->len == 0 || is_shared(b))
     return 0;
   for (int i = 0; i < tm->ndim; ++i)
     if (tm->shape[i] != ta->shape[ta->ndim - tm->ndim + i]) return 0;
@@ -251,7 +256,7 @@ GemmOperand operand_of(int64_t h, size_t nz, size_t rows, size_t cols) {
   o.z = v.d[0];
   o.r = v.d[1];
   o.c = v.d[2];
-  o.key = t->st->id;
+  o.key = t->st->shared ? 0 : t->st->id;
   return o;
 }
 

@@ -912,6 +912,10 @@ int32_t malus_tensor_dtype(int64_t h) { return tb(h)->dtype; }
 int32_t malus_tensor_describe(int64_t h, int64_t* out) {
   const auto* t = tb(h);
   out[0] = reinterpret_cast<int64_t>(malus_tensor_data(h));
+  if (!t->st->shared) {   // the caller may write through the pointer, now and later
+    t->st->shared = true;
+    plane_cache_drop(t->st->id);
+  }
   out[1] = t->dtype;
   out[2] = t->ndim;
   for (int i = 0; i < t->ndim; ++i) out[3 + i] = (int64_t)t->shape[i];
@@ -943,6 +947,11 @@ int64_t malus_tensor_wrap(int32_t dtype, void* dev_ptr, const size_t* shape, siz
   size_t n = 1;
   for (size_t i = 0; i < ndims; ++i) n *= shape[i];
   return make_handle(dtype, shape, (int)ndims, st, n);
+}
+int64_t malus_tensor_wrap_shared(int32_t dtype, void* dev_ptr, const size_t* shape, size_t ndims) {
+  const int64_t h = malus_tensor_wrap(dtype, dev_ptr, shape, ndims);
+  tb(h)->st->shared = true;
+  return h;
 }
 void malus_set_device(int32_t dev) {
   if (g_ctx.init) {
