@@ -309,7 +309,8 @@ int32_t malus_linear_xent_mode(int32_t mode);
 /* Distillation from a teacher's top logits: logits [N, V], and per row K <= 1024
  * entries ids [N, K] with teacher logits [N, K].  p = softmax over the row's
  * entries of teacher / temperature, q = softmax(logits / temperature); kl [N]
- * is temperature^2 * sum p (log p - log q) and the loss [1] its mean over the
+ * is temperature^2 * sum p (log p - log q) (temperature: 2^-60 to 2^60) and the loss
+ * [1] its mean over the
  * counted rows, those with an entry.  A negative id, or a teacher logit of
  * -inf, is no entry (an id at or past V is treated so too, and reported
  * through malus_device_error as 4); an id listed twice counts as both entries.

@@ -984,6 +984,8 @@ int64_t malus_distill(int64_t logits, int64_t ids, int64_t teacher, float temper
   if (!same_shape(ids, teacher)) panic("distill ids and teacher logits must have the same shape");
   if (!(temperature > 0.0f) || !std::isfinite(temperature))
     panic("distill temperature must be positive and finite, got %g", (double)temperature);
+  if (temperature < 0x1p-60f || temperature > 0x1p60f)   // its square and its inverse stay floats
+    panic("distill temperature must lie between 2^-60 and 2^60, got %g", (double)temperature);
   const int64_t n = (int64_t)s.d[0], V = (int64_t)s.d[1], K = (int64_t)si.d[1];
   if (V == 0) panic("distill over an empty vocabulary");
   if (K < 1 || K > kMaxEntries) panic("distill takes 1 to %d teacher entries per row, got %lld", kMaxEntries, (long long)K);
