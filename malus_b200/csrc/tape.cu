@@ -482,8 +482,10 @@ void backward(int64_t loss) {
         for (size_t i = 0; i < k; ++i) {
           int64_t in = n.saved[i], g = n.saved[k + i];
           if (!need(in)) continue;
-          // against the seed of ones the saved gradient is the result
-          accumulate(grads, in, dout == seed ? alias_of(g) : __broadcast_mul_fwd(g, dout));
+          // against the seed of ones the saved gradient is the result; but a registered
+          // leaf's is averaged over the ranks in place, which its other holders must not see
+          const bool written = dp && dp_is_leaf(in) && (tb(g)->rc.load() > 1 || (tb(g)->st && tb(g)->st->aliases > 1));
+          accumulate(grads, in, dout == seed && !written ? alias_of(g) : __broadcast_mul_fwd(g, dout));
         }
         break;
       }
