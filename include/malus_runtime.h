@@ -298,7 +298,11 @@ void malus_layernorm_affine_bwd(int64_t x, int64_t weight, int64_t stats, int64_
  * gradient (a target at or past V is treated so too, and reported through
  * malus_device_error as 4).  Without counted rows the loss is 0.  dx and
  * dweight are the gradients of the loss (for dout = 1; see tape_record_loss).
- * V is limited to 2^24. */
+ * V is limited to 2^24.  x and weight are to be finite in the counted rows (a value
+ * that is not may make any result NaN); rows that are not counted may hold anything.
+ * Workspace: 8 B per element of x and of weight, and 512 MB of logits, or 64 rows of
+ * them where that is more (from V = 2^21 on), twice over when both gradients are
+ * wanted; the loss alone keeps no logits. */
 int64_t malus_linear_xent(int64_t x, int64_t weight, int64_t targets, int32_t tied, int64_t* nll, int64_t* dx,
                           int64_t* dweight);
 /* Which products malus_linear_xent uses in the calling thread: -1 (default) the
@@ -309,9 +313,9 @@ int32_t malus_linear_xent_mode(int32_t mode);
 /* Distillation from a teacher's top logits: logits [N, V], and per row K <= 1024
  * entries ids [N, K] with teacher logits [N, K].  p = softmax over the row's
  * entries of teacher / temperature, q = softmax(logits / temperature); kl [N]
- * is temperature^2 * sum p (log p - log q) (temperature: 2^-60 to 2^60) and the loss
- * [1] its mean over the
- * counted rows, those with an entry.  A negative id, or a teacher logit of
+ * is temperature^2 * sum p (log p - log q), temperature within 2^-60 and 2^60, and
+ * the loss [1] its mean over the counted rows, those with an entry.  A negative id,
+ * or a teacher logit of
  * -inf, is no entry (an id at or past V is treated so too, and reported
  * through malus_device_error as 4); an id listed twice counts as both entries.
  * dlogits is the gradient of the loss (for dout = 1).  V is limited to 2^24. */

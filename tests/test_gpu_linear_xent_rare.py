@@ -55,3 +55,38 @@ def test_rows_of_rare_entries(M, rt, mode, n, D, V, tied):  # noqa: F811
     bad = ~(np.abs(dw - want) <= tol + 1e-36)
     assert not bad.any(), f"{bad.any(1).sum()} of {V} rows off, worst {np.max(np.abs(dw - want) / (tol + 1e-36)):.3g}"
     assert rt.malus_device_error() == 0
+
+
+@pytest.mark.parametrize("tied", [True, False])
+def test_a_vocabulary_past_the_piece_bound(M, rt, tied):
+    """over 2^21 entries a piece is 64 rows whatever its size: two pieces here, the second
+    of six rows, formula and tolerances as above, ten rows at a time"""
+    n, D, V = 70, 8, (1 << 21) + 1001
+    x, w, t = inputs(n, D, V, 1)
+    loss, nll, dx, dw = run(M, x, w, t, tied)
+    assert rt.malus_device_error() == 0
+    X, W = x.astype(np.float64), w.astype(np.float64)
+    cnt = int((t >= 0).sum())
+    want, tol, largest = np.zeros((V, D)), np.zeros((V, D)), np.zeros(V)
+    for r0 in range(0, n, 10):
+        s = slice(r0, r0 + 10)
+        ok = t[s] >= 0
+        z = X[s] @ W.T
+        m = z.max(1, keepdims=True)
+        z -= m
+        lse = np.log(np.exp(z).sum(1, keepdims=True))
+        zt = z[np.arange(10), np.where(ok, t[s], 0)]
+        assert (np.abs(nll[s] - np.where(ok, lse[:, 0] - zt, 0)) <= U * (100 + 12 * np.abs(zt))).all()
+        q = np.exp(z - lse) * ok[:, None]
+        edl = q * U * (80 + 8 * np.abs(z))
+        q[np.arange(10)[ok], t[s][ok]] -= 1
+        edl += 2 * U * np.abs(q)
+        ad, ax = np.abs(q), np.abs(X[s])
+        want += q.T @ X[s] / cnt
+        tol += (edl.T @ ax + (ad.T @ ax) * (99 * 2.0 ** -23 + 8 * U) + 2.0 ** -39 * 2 * ad.sum(0)[:, None]) / cnt
+        largest = np.maximum(largest, ad.max(0))
+        tx = (edl @ np.abs(W) + (99 + V / 512) * 2.0 ** -23 * (ad @ np.abs(W)) + 2.0 ** -39 *
+              (ad.max(1)[:, None] * np.abs(W).sum(0) + ad.sum(1)[:, None] * np.abs(W).max(0))) / cnt
+        assert (np.abs(dx[s] - q @ W / cnt) <= tx * 1.001 + 1e-36).all()
+    tol += 2.0 ** -39 * largest[:, None] * np.abs(X).sum(0) / cnt
+    assert (np.abs(dw - want) <= tol + 1e-36).all()
