@@ -322,36 +322,38 @@ RowCfg row_cfg(int64_t D, int most) {
   return {tpr, (int)((D + 4 * tpr - 1) / (4 * tpr))};
 }
 
-// 64 and 128 threads never hold more than 6 groups each.
-template <int TPR, bool VEC, class F>
-void with_nv(int nv, F&& f) {
-  constexpr int kMost = TPR == 64 || TPR == 128 ? 6 : 8;
-  switch (nv) {
-    case 1: f.template operator()<TPR, 1, VEC>(); break;
-    case 2: f.template operator()<TPR, 2, VEC>(); break;
-    case 3: f.template operator()<TPR, 3, VEC>(); break;
-    case 4: f.template operator()<TPR, 4, VEC>(); break;
-    case 5: f.template operator()<TPR, 5, VEC>(); break;
-    case 6: f.template operator()<TPR, 6, VEC>(); break;
-    case 7: f.template operator()<TPR, std::min(7, kMost), VEC>(); break;
-    default: f.template operator()<TPR, std::min(8, kMost), VEC>(); break;
-  }
+// Whether row_cfg(D, MOST) ever gives NV groups with TPR threads: only those exist.
+template <int MOST>
+constexpr bool reached(int tpr, int nv) {
+  if (tpr == 8) return nv <= MOST;
+  if (tpr == 16) return nv > MOST / 2 && nv <= MOST;
+  if (tpr == 32) return nv > MOST / 2 && nv <= 8;   // to 1024 elements
+  if (tpr == 64) return nv == 5 || nv == 6;         // from 1025 on
+  return nv >= 4 && nv <= (tpr == 128 ? 6 : 8);
 }
-template <bool VEC, class F>
+template <int MOST, int TPR, bool VEC, int NV = 1, class F>
+void with_nv(int nv, F&& f) {
+  if constexpr (NV <= 8) {
+    if (nv != NV) return with_nv<MOST, TPR, VEC, NV + 1>(nv, f);
+    if constexpr (reached<MOST>(TPR, NV)) return f.template operator()<TPR, NV, VEC>();
+  }
+  panic("layernorm_affine: no kernel of %d threads per row and %d groups", TPR, nv);
+}
+template <int MOST, bool VEC, class F>
 void with_tpr(RowCfg c, F&& f) {
   switch (c.tpr) {
-    case 8: with_nv<8, VEC>(c.nv, f); break;
-    case 16: with_nv<16, VEC>(c.nv, f); break;
-    case 32: with_nv<32, VEC>(c.nv, f); break;
-    case 64: with_nv<64, VEC>(c.nv, f); break;
-    case 128: with_nv<128, VEC>(c.nv, f); break;
-    default: with_nv<256, VEC>(c.nv, f); break;
+    case 8: with_nv<MOST, 8, VEC>(c.nv, f); break;
+    case 16: with_nv<MOST, 16, VEC>(c.nv, f); break;
+    case 32: with_nv<MOST, 32, VEC>(c.nv, f); break;
+    case 64: with_nv<MOST, 64, VEC>(c.nv, f); break;
+    case 128: with_nv<MOST, 128, VEC>(c.nv, f); break;
+    default: with_nv<MOST, 256, VEC>(c.nv, f); break;
   }
 }
-template <class F>
-void with_cfg(RowCfg c, bool vec, F&& f) {
-  if (vec) with_tpr<true>(c, f);
-  else with_tpr<false>(c, f);
+template <int MOST, class F>
+void with_cfg(int64_t D, bool vec, F&& f) {
+  if (vec) with_tpr<MOST, true>(row_cfg(D, MOST), f);
+  else with_tpr<MOST, false>(row_cfg(D, MOST), f);
 }
 
 struct FwdLaunch {
@@ -410,7 +412,7 @@ void norm_affine_fwd(const float* x, const float* w, const float* b, float* y, f
   } else {
     const bool vec = D % 4 == 0 && aligned16({x, w, b, y});
     const FwdLaunch f{x, w, b, y, stats, rows, (int)D, eps};
-    with_cfg(row_cfg(D, kFwdNv), vec, f);
+    with_cfg<kFwdNv>(D, vec, f);
   }
   count_launch();
   after_launch("k_norm_fwd");
@@ -440,7 +442,7 @@ void norm_affine_bwd(const float* x, const float* w, const float* stats, const f
     }
   } else {
     const bool vec = D % 4 == 0 && aligned16({x, w, dy, dx});
-    with_cfg(row_cfg(D, kBwdNv), vec, BwdLaunch{x, w, stats, dy, dx, dw, db, rows, (int)D});
+    with_cfg<kBwdNv>(D, vec, BwdLaunch{x, w, stats, dy, dx, dw, db, rows, (int)D});
     count_launch();
   }
   after_launch("k_norm_bwd");
