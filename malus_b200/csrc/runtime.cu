@@ -938,6 +938,11 @@ void malus_tensor_write(int64_t h, const void* src, size_t bytes) {
   gpu_barrier();
 }
 int64_t malus_tensor_wrap(int32_t dtype, void* dev_ptr, const size_t* shape, size_t ndims) {
+  if (dtype != MALUS_F32 && dtype != MALUS_I32 && dtype != MALUS_I64)
+    panic("unsupported dtype tag %d; supported: f32, i32, i64", dtype);
+  if (ndims > (size_t)kMaxRank) panic("rank %zu exceeds the maximum of %d", ndims, kMaxRank);
+  if (reinterpret_cast<uintptr_t>(dev_ptr) % dtype_size(dtype))
+    panic("malus_tensor_wrap: address %p is not aligned to its elements of %zu bytes", dev_ptr, (size_t)dtype_size(dtype));
   auto* st = new Storage();
   st->ptr = dev_ptr;
   st->bytes = 0;
