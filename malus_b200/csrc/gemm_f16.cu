@@ -669,9 +669,12 @@ __global__ void __launch_bounds__(256) k_split_cols(const SplitJobs jobs, int64_
     for (int i = 0; i < 16; ++i, q += 4 * C) v[i] = ty + 4 * i < nr && tx < nc ? *q : 0.0f;
   }
   if (t < 64) {
-    const bool k = t < nr && kept(job.keep, job.keep_dtype, job.limit, r0 + t);
+    const bool k = t < nr && kept(job.keep, job.keep_dtype, job.limit, r0 + t, jobs.count && c0 == 0 ? jobs.err : nullptr);
     const uint32_t b = __ballot_sync(0xffffffffu, k);
-    if ((t & 31) == 0) rows_kept[t >> 5] = b;
+    if ((t & 31) == 0) {
+      rows_kept[t >> 5] = b;
+      if (which == 0 && jobs.count && c0 == 0 && b) atomicAdd(jobs.count, __popc(b));
+    }
     float up = 1.0f, iv = 1.0f;
     if (t < nc) f16_scale(bits[c0 + t], &up, &iv);
     ups[t] = up;
@@ -912,11 +915,13 @@ void split_cols(SplitJobs jobs, int n, int64_t C, bool vec) {
 
 }  // namespace
 
-void f16_split_cols(const F16Split& job, int64_t C) {
+void f16_split_cols(const F16Split& job, int64_t C, int* count) {
   if (C == 0 || job.R == 0) return;
   const int pid = prof_begin(1, 0.0, 8.0 * (double)job.R * (double)C);
   SplitJobs jobs{};
   jobs.j[0] = job;
+  jobs.count = count;
+  jobs.err = device_error_word();
   jobs.bits[0] = static_cast<uint32_t*>(scratch_alloc((size_t)C * 4));
   MALUS_CUDA(cudaMemsetAsync(jobs.bits[0], 0, (size_t)C * 4, stream()));
   col_max(job.src, job.R, C, jobs.bits[0], job.keep, job.keep_dtype, job.limit);
@@ -925,7 +930,7 @@ void f16_split_cols(const F16Split& job, int64_t C) {
   prof_end(pid);
 }
 
-bool f16_split_both(const F16Split* job, int n, int64_t C, uint32_t* bits, int* count) {
+void f16_split_both(const F16Split* job, int n, int64_t C, uint32_t* bits, int* count) {
   // one read for the rows' planes and the columns' maxima where a warp's registers
   // hold a row: 50304 x 768 measured 47 us (the copy rate) against 52 and 33 apart
   bool fit = C <= 1024 && C % 4 == 0;
@@ -937,9 +942,9 @@ bool f16_split_both(const F16Split* job, int n, int64_t C, uint32_t* bits, int* 
   if (!fit) {
     for (int i = 0; i < n; ++i) {
       f16_split_rows(job[i].src, job[i].R, C, job[i].rhi, job[i].rlo, job[i].rinv);
-      f16_split_cols(job[i], C);
+      f16_split_cols(job[i], C, i == 0 ? count : nullptr);
     }
-    return false;
+    return;
   }
   const int pid = prof_begin(1, 0.0, bytes);
   SplitJobs jobs{};
@@ -974,9 +979,9 @@ bool f16_split_both(const F16Split* job, int n, int64_t C, uint32_t* bits, int* 
   }
   count_launch();
   after_launch("k_split_rows_max");
+  jobs.count = nullptr;   // they are counted
   split_cols(jobs, n, C, true);
   prof_end(pid);
-  return true;
 }
 
 }  // namespace malus

@@ -65,11 +65,11 @@ struct F16Split {
   int64_t limit;
 };
 void f16_split_rows(const float* src, int64_t R, int64_t C, __half* hi, __half* lo, float* inv);
-void f16_split_cols(const F16Split& job, int64_t C);
+// With count (zero before), here and below: count[0] has the first matrix's kept rows
+// after it, and ids at or past its limit are reported in the error word.
+void f16_split_cols(const F16Split& job, int64_t C, int* count = nullptr);
 // Both of one or two matrices (R > 0) of C columns.  bits: n * C words, zero.
-// Returns whether count[0] (zero before) now has the first one's kept rows, and ids
-// at or past its limit are reported in the error word.
-bool f16_split_both(const F16Split* jobs, int n, int64_t C, uint32_t* bits, int* count);
+void f16_split_both(const F16Split* jobs, int n, int64_t C, uint32_t* bits, int* count);
 __host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // floats behind the scales of `rows` plane rows: a GEMM reads whole tiles of them

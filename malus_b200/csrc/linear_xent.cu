@@ -66,18 +66,17 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
   const F16Split sx{x, n, xr.hi, xr.lo, xr.inv, xc.hi, xc.lo, xc.inv, tgt, tdt, V};
   const F16Split sw = tied ? F16Split{w, V, wv.hi, wv.lo, wv.inv, wd.hi, wd.lo, wd.inv, nullptr, 0, 0}
                            : F16Split{w, D, wd.hi, wd.lo, wd.inv, wv.hi, wv.lo, wv.inv, nullptr, 0, 0};
-  bool counted = false;
   if (dw && dx && tied) {
     const F16Split both[2] = {sx, sw};
-    counted = f16_split_both(both, 2, D, bits, count);
+    f16_split_both(both, 2, D, bits, count);
   } else {
-    if (dw) counted = f16_split_both(&sx, 1, D, bits, count);
+    if (dw) f16_split_both(&sx, 1, D, bits, count);
     else f16_split_rows(x, n, D, xr.hi, xr.lo, xr.inv);
     if (dx) f16_split_both(&sw, 1, tied ? D : V, bits + D, nullptr);
     else if (tied) f16_split_rows(w, V, D, wv.hi, wv.lo, wv.inv);
     else f16_split_cols(sw, V);
   }
-  if (!counted) xent_count(tgt, tdt, n, V, count);
+  if (!dw) xent_count(tgt, tdt, n, V, count);
   // Pieces of whole 256-row tiles, of even size; of 64 rows (the products' step in K)
   // where 256 do not fit the bound.
   const int64_t fit = (int64_t)(kPieceBytes / ((size_t)ld * 4));
