@@ -168,7 +168,7 @@ __device__ __forceinline__ void finish_lse(const Params& p, float (&acc)[kCols],
   float s = 0.0f;
   const float mm = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) s += exp2f((acc[j] - mm) * kLog2e);
+  for (int j = 0; j < kCols; ++j) s += exp2_hw((acc[j] - mm) * kLog2e);
   p.part[(int64_t)m * (BN / kCols * p.tiles_n) + n0 / kCols] = make_float2(mx, s);
   const int64_t t = p.tdt == MALUS_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
   if (t >= n0 && t < n0 + kCols && t < p.N) {
@@ -359,33 +359,20 @@ k_gemm_f16(const __grid_constant__ CUtensorMap mAh, const __grid_constant__ CUte
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if constexpr (MODE == kByM || MODE == kByN) {
+        const bool first = st == un.st_lo;
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(tbase + b * BN + c, r);
+        for (int c = 0; c < kCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(tbase + b * BN + c, r);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              float4 s = make_float4(bm, bm, bm, bm);
-              if (MODE == kByN) s = scale4(make_float4(1.0f, 1.0f, 1.0f, 1.0f), 1.0f, bn, (c + j) / 4);
-              float* a = acc + c + j;
-              const bool first = st == un.st_lo;
-              a[0] = fmaf(__uint_as_float(r[j]), s.x, first ? 0.0f : a[0]);
-              a[1] = fmaf(__uint_as_float(r[j + 1]), s.y, first ? 0.0f : a[1]);
-              a[2] = fmaf(__uint_as_float(r[j + 2]), s.z, first ? 0.0f : a[2]);
-              a[3] = fmaf(__uint_as_float(r[j + 3]), s.w, first ? 0.0f : a[3]);
-            }
-          }
-        } else if (st == un.st_lo) {
-#pragma unroll
-          for (int c = 0; c < kCols; c += 32) tmem_ld32(tbase + b * BN + c, reinterpret_cast<uint32_t*>(acc + c));
-        } else {
-#pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(tbase + b * BN + c, r);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(r[j]);
+          for (int j = 0; j < 32; j += 4) {
+            float4 s = make_float4(bm, bm, bm, bm);
+            if (MODE == kByN) s = scale4(make_float4(1.0f, 1.0f, 1.0f, 1.0f), 1.0f, bn, (c + j) / 4);
+            float* a = acc + c + j;
+            a[0] = fmaf(__uint_as_float(r[j]), s.x, first ? 0.0f : a[0]);
+            a[1] = fmaf(__uint_as_float(r[j + 1]), s.y, first ? 0.0f : a[1]);
+            a[2] = fmaf(__uint_as_float(r[j + 2]), s.z, first ? 0.0f : a[2]);
+            a[3] = fmaf(__uint_as_float(r[j + 3]), s.w, first ? 0.0f : a[3]);
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
