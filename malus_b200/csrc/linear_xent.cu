@@ -101,7 +101,7 @@ void train(const float* x, const float* w, const void* tgt, int tdt, bool tied, 
     gemm_f16_lse(g, part, at, t, tdt);
     xent_planes(logits, ld, m, V, {part, parts, at, t, tdt}, nll + r0, even, entry, inv, inv_pitch);
     if (dx) {
-      const F16Operand dl{even, even + 64, m, ld, 2 * ld, false, 0, nullptr, 1.0f / (1 << kF16Exp), true};
+      const F16Operand dl{even, even + 64, m, ld, 2 * ld, false, 0, nullptr, 1.0f / (1 << kDlExp), true};
       gemm_f16({(int)m, (int)D, (int)V, dl, wd.kmajor(0, D), dx + r0 * D, D, false, count});
     }
     if (dw) {

@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(256) k_xent_join(const XentParts p, int64_t V,
 // softmax - onehot, in the grouped layout of F16Operand, in one pass: 4 B read per
 // logit and 4 B written per set of planes (2048 x 50304, both sets: 197 us, 6.3 TB/s; with
 // 256 threads of 16 groups each 265 us).  EVEN: at one scale,
-// 2^kF16Exp, for a product that sums over the vocabulary, where the largest of a
+// 2^kDlExp, for a product that sums over the vocabulary, where the largest of a
 // token's gradients sets the accuracy.  ENTRY: scaled per vocabulary entry by the
 // largest of its column in the tile, for the product that sums over the tokens:
 // there each entry's row of dweight has a size of its own, from 1 down to the
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kTileThreads, 1024 / kTileThreads)
 k_xent_planes(const float* logits, int64_t ld, int64_t n, int64_t V, const XentStat* __restrict__ stat, const XentParts p,
               float* __restrict__ nll, __half* even, __half* entry, float* __restrict__ inv, int64_t inv_pitch) {
   constexpr int kStep = kTileThreads / 16, kRows = kF16Block / kStep, kTileWarps = kTileThreads / 32;
-  constexpr float one = (float)(1 << kF16Exp);
+  constexpr float one = (float)(1 << kDlExp);
   __shared__ XentStat st[kF16Block];
   __shared__ __align__(16) float sh[kTileWarps][64], ups[64];
   const int groups = (int)(ld / 64), g = (int)(blockIdx.x % groups), tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -358,7 +358,7 @@ k_xent_planes(const float* logits, int64_t ld, int64_t n, int64_t V, const XentS
       q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       continue;
     }
-    const float f = s.inv_sum * one;   // dl times 2^kF16Exp
+    const float f = s.inv_sum * one;   // dl times 2^kDlExp
     q[i].x = tc::exp2_hw((q[i].x - s.max) * kLog2e) * f;
     q[i].y = tc::exp2_hw((q[i].y - s.max) * kLog2e) * f;
     q[i].z = tc::exp2_hw((q[i].z - s.max) * kLog2e) * f;

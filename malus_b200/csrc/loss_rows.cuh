@@ -30,9 +30,11 @@ struct __align__(16) XentStat {
 // nll[r], and stat[r] where not null
 void xent_join(const XentParts& p, int64_t V, int64_t n, float* nll, XentStat* stat);
 
+constexpr int kDlExp = 15;   // magnitudes of softmax - onehot are at most 1: 2^15 is half's last power of two
+
 // nll[r], and half planes of softmax - onehot, from n > 0 rows of f32 logits (row pitch
 // ld >= V, a multiple of 64; what lies from V on is not looked at), in the grouped
-// layout with a pitch of 2 ld halves: `even` all at 2^kF16Exp; `entry` scaled per
+// layout with a pitch of 2 ld halves: `even` all at 2^kDlExp; `entry` scaled per
 // kF16Block rows and vocabulary entry, with the inverse scales in inv (rows of
 // inv_pitch >= ld floats).  Either may be null, not both, and one of them may lie over
 // the logits.
