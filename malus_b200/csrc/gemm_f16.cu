@@ -759,8 +759,8 @@ void launch(const F16Gemm& g, Params& p, float* out, int64_t ldo, int64_t sstrid
   p.inv_all = (g.a.inv ? 1.0f : g.a.inv_all) * (g.b.inv ? 1.0f : g.b.inv_all);
   p.err = device_error_word();
   const int units = p.tiles_m * p.tiles_n * p.splits;
-  // half the chain where it costs nothing (16384 x 384 x 65, three products: 60 us
-  // either way; 2048 x 768 x 50304: 377 us with 4, 472 with 2)
+  // half the chain where it costs little (16384 x 384 x 65, three products: 59 us, 57
+  // with 4; 2048 x 768 x 50304: 360 us with 4, 418 with 2)
   p.chunk = units <= max_pairs() && (p.nst + p.splits - 1) / p.splits <= kShortUnit ? kShortChunk : kChunk;
   // a chunk lies within one block of scales
   p.align = MODE == kByM || MODE == kByN ? p.chunk : 1;

@@ -231,12 +231,12 @@ void launch(const Small& s) {
 
 }  // namespace
 
-// Measured against half planes, the whole call: training 128 x 181 x 1586 45 us
-// against 99, 256 x 384 x 1000 (9.8e7) 60 against 72, 256 x 768 x 1000 (2.0e8) 84
-// against 75; and 100 x 100 x 10000 (1.3e8) 119 against 78, 16384 x 64 x 64 (6.7e7)
-// 147 against 79, where a gradient sums over more than its slices can hide.  The
+// Measured against half planes, the whole call: training 128 x 181 x 1586 43 us
+// against 93, 256 x 384 x 1000 (9.8e7) 59 against 76, 256 x 768 x 1000 (2.0e8) 83
+// against 82; and 100 x 100 x 10000 (1.3e8) 118 against 77, 16384 x 64 x 64 (6.7e7)
+// 146 against 78, where a gradient sums over more than its slices can hide.  The
 // loss alone sums over D only: 64 x 384 x 2000 (4.9e7) 23 against 33, 256 x 384 x
-// 1000 (9.8e7) 31 against 32, 1000 x 384 x 500 (2.0e8) 46 against 32.
+// 1000 (9.8e7) 30 against 33, 1000 x 384 x 500 (2.0e8) 45 against 33.
 bool head_small(int64_t n, int64_t D, int64_t V, bool grad) {
   const double rows = n <= 16 ? 16.0 : (double)((n + 63) / 64 * 64);   // of x, padded to the tile
   const double work = rows * (double)D * (double)V;

@@ -1,10 +1,11 @@
-// Softmax losses by rows: the cross entropy of a logits row against its target
-// (for the head, linear_xent.cu), and distillation from a teacher's top logits:
+// Softmax losses by rows: for the head (linear_xent.cu) the cross entropy of a logits
+// row against its target, and half planes of its gradient by tiles (k_xent_planes); and
+// distillation from a teacher's top logits:
 //
 //   p = softmax over the row's entries of teacher / T,  q = softmax(logits / T)
 //   kl = T^2 sum_k p_k (log p_k - log q[id_k]),  dlogits = T (q - p) / rows
 //
-// Bound by HBM: 4 B read and 4 B written per logit.  Rows up to 1020 logits take
+// Rows, bound by HBM: 4 B read and 4 B written per logit.  Rows up to 1020 logits take
 // a warp each, held in registers.  Longer ones take a block that stays and walks
 // rows through a ring of shared-memory chunks: one warp feeds the ring by bulk
 // copies, the others pass over a row twice, maximum and sum of exponentials first,
