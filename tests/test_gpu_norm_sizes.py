@@ -7,8 +7,9 @@ from test_gpu_norm_affine import inputs, reference, run, within
 
 pytestmark = pytest.mark.gpu
 
-EDGES = sorted({e + o for step, top in ((32, 128), (32, 256), (64, 512), (128, 1024), (256, 1536), (512, 3072), (1024, 8192))
-                for e in range(step, top + 1, step) for o in (-3, -1, 0, 1, 4) if 1 <= e + o <= 8196})
+STEPS = ((32, 128), (32, 256), (64, 512), (128, 1024), (256, 1536), (512, 2560), (1024, 8192))   # of a class, its last length
+EDGES = sorted({e + o for step, top in STEPS for e in range(step, top + 1, step) for o in (-3, -1, 0, 1, 4)
+                if e != 3 * 1024 and 1 <= e + o <= 8196} | {3069, 3071, 3073, 3076})   # 128 threads' last, 256 threads' first
 
 
 @pytest.mark.parametrize("part", range(4))
