@@ -160,7 +160,8 @@ void* malus_tensor_data(int64_t h);
 int32_t malus_tensor_dtype(int64_t h);
 /* All of the above in one call: out = (data pointer, dtype, rank, shape...), 11
  * words at most; returns the rank.  From then on the memory is shared, as
- * malus_tensor_wrap_shared says. */
+ * malus_tensor_wrap_shared says; a product of it deferred before is still computed
+ * when it is first read. */
 int32_t malus_tensor_describe(int64_t h, int64_t* out);
 /* Copy a tensor to / from host memory (synchronous). */
 void malus_tensor_read(int64_t h, void* dst, size_t bytes);

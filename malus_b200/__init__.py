@@ -305,7 +305,9 @@ class Tensor:
         """The data for another library on the same GPU, without a copy.  It is
         written on the runtime's stream: wait for that (gpu_barrier) before
         reading it on another, and keep this object alive meanwhile.  Writes to it
-        are seen by the calls that follow them (wait for the writing stream first)."""
+        are seen by the calls that follow them (wait for the writing stream first),
+        and by views of it and products of it that were made before this was first
+        read and are still deferred."""
         d = _DESCRIBE()
         n = load().malus_tensor_describe(self.h, d)
         shape = tuple(d[3:3 + n])

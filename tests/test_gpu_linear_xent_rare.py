@@ -8,6 +8,8 @@ and sum of the logits is exact, so log q carries only the softmax's own error,
 (80 + 8 |z - max|) u as in the distillation tests, and dl = q - onehot that error
 of q and two roundings.  No absolute error is allowed for: the products' bound
 (prod_tol) is relative to the terms and to the largest one of the row."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -90,3 +92,19 @@ def test_a_vocabulary_past_the_piece_bound(M, rt, tied):
         assert (np.abs(dx[s] - q @ W / cnt) <= tx * 1.001 + 1e-36).all()
     tol += 2.0 ** -39 * largest[:, None] * np.abs(X).sum(0) / cnt
     assert (np.abs(dw - want) <= tol + 1e-36).all()
+
+
+@pytest.mark.parametrize("tied", [True, False])
+def test_one_gradient_alone_over_several_pieces(M, rt, tied):
+    """with one gradient the planes lie over the logits, with both only dweight's do: the
+    same bits either way, over two pieces"""
+    x, w, t = inputs(2700, 16, 50304, 3)
+    T = M.Tensor.from_numpy
+    tx, tw, tt = T(x), T(w if tied else np.ascontiguousarray(w.T)), T(t)
+    loss, nll, dx, dw = M.linear_xent(tx, tw, tt, tied=tied)
+    for i, both in ((1, dx), (2, dw)):
+        out = [(C.c_int64 * 1)() for _ in range(3)]
+        rt.tensor_release(rt.malus_linear_xent(tx.h, tw.h, tt.h, int(tied), out[0], *(out[k] if k == i else None for k in (1, 2))))
+        got = [M.Tensor(out[0][0]), M.Tensor(out[i][0])]
+        assert np.array_equal(got[0].numpy(), nll.numpy()) and np.array_equal(got[1].numpy(), both.numpy())
+    assert rt.malus_device_error() == 0
